@@ -19,10 +19,12 @@ SWA_ERR_LAUNCH = 3
 SWA_ERR_DEVICE_TIMEOUT = 4
 SWA_ERR_WORKSPACE = 5
 SWA_ERR_TOO_LARGE = 6
+SWA_ERR_BAD_PAGE = 7
 SWA_NO_ALLOC_SCRATCH_BYTES = 16 << 20
 
 SWA_F16 = 0
 SWA_BF16 = 1
+SWA_ROTARY_MAX_FREQS = 64
 
 # Every extern "C" symbol include/swa_attn.h declares.
 EXPORTED_SYMBOLS = (
@@ -32,6 +34,8 @@ EXPORTED_SYMBOLS = (
     "swa_selftest_wait_timeout", "swa_fwd_sink_logits", "swa_bwd_sink_logits",
     "swa_varlen_lse_floats", "swa_varlen_bwd_workspace_size", "swa_varlen_fwd", "swa_varlen_bwd",
     "swa_device_status_async",
+    "swa_rotary", "swa_paged_append", "swa_paged_decode", "swa_paged_decode_workspace_size",
+    "swa_paged_evict", "swa_paged_evict_workspace_size",
 )
 
 
@@ -79,6 +83,58 @@ class SwaVarlenBwdArgs(ctypes.Structure):
                 ("workspace_bytes", ctypes.c_size_t)]
 
 
+class SwaRotary(ctypes.Structure):
+    _fields_ = [("inv_freq", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+                ("pos_stride_axis", ctypes.c_int64), ("pos_stride_b", ctypes.c_int64),
+                ("pos_stride_l", ctypes.c_int64), ("pos_is_64", ctypes.c_int32),
+                ("n_axes", ctypes.c_int32), ("n_freq", ctypes.c_int32),
+                ("interleaved", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("axis", ctypes.c_uint8 * SWA_ROTARY_MAX_FREQS)]
+
+
+class SwaRotaryArgs(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int32), ("n_q_heads", ctypes.c_int32),
+                ("n_kv_heads", ctypes.c_int32), ("seq_len", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("inverse", ctypes.c_int32), ("r", SwaRotary), ("q", SwaTensor), ("k", SwaTensor),
+                ("q_out", SwaTensor), ("k_out", SwaTensor)]
+
+
+class SwaPagedKV(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + \
+        [(f"{x}_stride_{y}", ctypes.c_int64) for x in "kv" for y in ("page", "head", "row")] + \
+        [("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+         ("seq_lens", ctypes.c_void_p), ("seen", ctypes.c_void_p), ("weights", ctypes.c_void_p),
+         ("positions", ctypes.c_void_p), ("w_stride_b", ctypes.c_int64),
+         ("w_stride_h", ctypes.c_int64), ("p_stride_b", ctypes.c_int64),
+         ("p_stride_h", ctypes.c_int64)] + \
+        [(n, ctypes.c_int32) for n in ("n_pages", "page_size", "max_pages", "batch", "n_kv_heads",
+                                       "head_dim", "dtype")]
+
+
+class SwaPagedAppendArgs(ctypes.Structure):
+    _fields_ = [("cache", SwaPagedKV), ("cu_new", ctypes.c_void_p), ("n_tokens", ctypes.c_int32),
+                ("n_q_heads", ctypes.c_int32), ("k", SwaPackedTensor), ("v", SwaPackedTensor),
+                ("q", SwaPackedTensor), ("q_out", SwaPackedTensor), ("use_rotary", ctypes.c_int32),
+                ("r", SwaRotary)]
+
+
+class SwaPagedDecodeArgs(ctypes.Structure):
+    _fields_ = [("cache", SwaPagedKV), ("n_q_heads", ctypes.c_int32),
+                ("window_size", ctypes.c_int32), ("sink_size", ctypes.c_int32),
+                ("softmax_scale", ctypes.c_float), ("q", SwaPackedTensor), ("o", SwaPackedTensor),
+                ("lse", ctypes.c_void_p), ("sink_logits", ctypes.c_void_p),
+                ("weights_out", ctypes.c_void_p), ("wo_stride_b", ctypes.c_int64),
+                ("wo_stride_h", ctypes.c_int64), ("decay", ctypes.c_float),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class SwaPagedEvictArgs(ctypes.Structure):
+    _fields_ = [("cache", SwaPagedKV), ("keep", ctypes.c_int32), ("trigger", ctypes.c_int32),
+                ("sink_size", ctypes.c_int32), ("recent", ctypes.c_int32),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
 class SwaError(RuntimeError):
     """A non-zero SwaStatus from the library."""
 
@@ -99,6 +155,7 @@ STATUS_NAMES = {
     SWA_ERR_UNSUPPORTED: "unsupported shape, dtype or layout", SWA_ERR_LAUNCH: "CUDA launch failed",
     SWA_ERR_DEVICE_TIMEOUT: "on-device wait timed out",
     SWA_ERR_WORKSPACE: "workspace missing, misaligned or too small",
+    SWA_ERR_BAD_PAGE: "page table entry or length out of range",
     SWA_ERR_TOO_LARGE: "problem needs more scratch than the static no-alloc workspace",
 }
 
@@ -125,6 +182,13 @@ def _declare(l):
     l.swa_varlen_fwd.restype = ctypes.c_int
     l.swa_varlen_bwd.argtypes = [P(SwaVarlenBwdArgs), ctypes.c_void_p]
     l.swa_varlen_bwd.restype = ctypes.c_int
+    for name, t in (("rotary", SwaRotaryArgs), ("paged_append", SwaPagedAppendArgs),
+                    ("paged_decode", SwaPagedDecodeArgs), ("paged_evict", SwaPagedEvictArgs)):
+        f = getattr(l, f"swa_{name}")
+        f.argtypes, f.restype = [P(t), ctypes.c_void_p], ctypes.c_int
+    for name, t in (("decode", SwaPagedDecodeArgs), ("evict", SwaPagedEvictArgs)):
+        f = getattr(l, f"swa_paged_{name}_workspace_size")
+        f.argtypes, f.restype = [P(t)], ctypes.c_size_t
     l.swa_bwd_workspace_size.argtypes = [P(SwaProblem)]
     l.swa_bwd_workspace_size.restype = ctypes.c_size_t
     for name in ("swa_bwd_dkdv_launch_count", "swa_bwd_launch_count"):
@@ -175,6 +239,23 @@ def check(status: int, where: str):
         detail = lib().swa_last_cuda_error().decode()
     cls = SwaDeviceTimeout if status == SWA_ERR_DEVICE_TIMEOUT else SwaError
     raise cls(status, where, detail)
+
+
+class _Same:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *a):
+        pass
+
+
+_SAME = _Same()
+
+
+def on_device(dev):
+    """Context in which ``dev`` is the current device (nothing to do where it already is)."""
+    import torch
+    return _SAME if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 # ---------------------------------------------------------------------------------------

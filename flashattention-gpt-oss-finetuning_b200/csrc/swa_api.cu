@@ -8,6 +8,7 @@
 #include <string>
 
 #include "swa_common.cuh"
+#include "swa_host.cuh"
 #include "swa_params.cuh"
 
 namespace swa {
@@ -32,21 +33,28 @@ thread_local std::string g_last_cuda_error;
 // copy).  Host code passes the device address obtained from cudaGetSymbolAddress.
 static __device__ int g_device_error;
 
+// Set by a paged-cache kernel that met a page or a length out of range (and did not follow it).
+static __device__ int g_page_error;
+
 constexpr int kMaxDev = 64;
 std::mutex g_err_mu;
 int* g_err_ptr[kMaxDev] = {};
+int* g_page_err_ptr[kMaxDev] = {};
 
-int* device_error_ptr() {
+// The current device's address of a flag, looked up once per device.
+int* flag_ptr(int** cache, const int& symbol) {
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDev) return nullptr;
   std::lock_guard<std::mutex> lock(g_err_mu);
-  if (!g_err_ptr[dev]) {
+  if (!cache[dev]) {
     void* p = nullptr;
-    if (cudaGetSymbolAddress(&p, g_device_error) != cudaSuccess) return nullptr;
-    g_err_ptr[dev] = static_cast<int*>(p);
+    if (cudaGetSymbolAddress(&p, symbol) != cudaSuccess) return nullptr;
+    cache[dev] = static_cast<int*>(p);
   }
-  return g_err_ptr[dev];
+  return cache[dev];
 }
+
+int* device_error_ptr() { return flag_ptr(g_err_ptr, g_device_error); }
 
 int record(cudaError_t e) {
   if (e == cudaSuccess) return SWA_OK;
@@ -242,6 +250,11 @@ int build_bwd(const SwaBwdArgs* a, swa::BwdParams* kp) {
 
 }  // namespace
 
+namespace swa {
+int host_record(cudaError_t e) { return record(e); }
+int* page_error_ptr() { return flag_ptr(g_page_err_ptr, g_page_error); }
+}  // namespace swa
+
 extern "C" {
 
 int swa_version(void) { return 100; }
@@ -257,6 +270,7 @@ const char* swa_status_string(int s) {
     case SWA_ERR_DEVICE_TIMEOUT: return "on-device wait timed out";
     case SWA_ERR_WORKSPACE: return "workspace missing, misaligned or too small";
     case SWA_ERR_TOO_LARGE: return "problem needs more scratch than the static no-alloc workspace";
+    case SWA_ERR_BAD_PAGE: return "page table entry or length out of range";
     default: return "unknown status";
   }
 }
@@ -269,11 +283,18 @@ int swa_check_device(void* stream) {
   int v = 0;
   e = cudaMemcpyFromSymbol(&v, g_device_error, sizeof(int));
   if (e != cudaSuccess) return record(e);
-  if (v == 0) return SWA_OK;
   const int zero = 0;
-  e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
+  if (v != 0) {
+    e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
+    if (e != cudaSuccess) return record(e);
+    return SWA_ERR_DEVICE_TIMEOUT;
+  }
+  e = cudaMemcpyFromSymbol(&v, g_page_error, sizeof(int));
   if (e != cudaSuccess) return record(e);
-  return SWA_ERR_DEVICE_TIMEOUT;
+  if (v == 0) return SWA_OK;
+  e = cudaMemcpyToSymbol(g_page_error, &zero, sizeof(int));
+  if (e != cudaSuccess) return record(e);
+  return SWA_ERR_BAD_PAGE;
 }
 
 int swa_device_status_async(int* host_flag, void* stream) {

@@ -230,10 +230,23 @@ class FlashSWDAWithSinkLogits(torch.autograd.Function):
         return dq, dk, dv, dsl.to(sinks.dtype), None, None, None, None
 
 
+def rotated(q, k, rotary, positions):
+    """q and k, turned by their positions where a rotation is given."""
+    if (rotary is None) != (positions is None):
+        raise ValueError("rotary and positions go together")
+    if rotary is None:
+        return q, k
+    from .rotary import apply_rotary  # rotary.py builds on this module
+    return apply_rotary(q, k, positions, rotary)
+
+
 def flash_swda_with_sink(q, k, v, window_size: int, sink_size: int = 0, is_causal: bool = True,
-                         scale: Optional[float] = None, sinks: Optional[torch.Tensor] = None):
+                         scale: Optional[float] = None, sinks: Optional[torch.Tensor] = None,
+                         rotary=None, positions: Optional[torch.Tensor] = None):
     """Same signature as the reference (flash_attention_gpt_oss.py:437-438), plus the
-    optional keyword ``sinks`` ([Hq] learned sink logits, see FlashSWDAWithSinkLogits)."""
+    optional keywords ``sinks`` ([Hq] learned sink logits, see FlashSWDAWithSinkLogits) and
+    ``rotary`` with ``positions`` (q and k are rotated first, see rotary.apply_rotary)."""
+    q, k = rotated(q, k, rotary, positions)
     if sinks is not None:
         return FlashSWDAWithSinkLogits.apply(q, k, v, sinks, window_size, sink_size, is_causal,
                                              scale)

@@ -21,7 +21,8 @@ import numpy as np
 import torch
 
 from . import _lib
-from .flash_attention_gpt_oss import (_DTYPES, _kernel_head_dim, _sink_logits_f32, _stream)
+from .flash_attention_gpt_oss import (_DTYPES, _kernel_head_dim, _sink_logits_f32, _stream,
+                                      rotated)
 
 CuSeqlens = Union[Sequence[int], torch.Tensor, np.ndarray]
 
@@ -180,8 +181,11 @@ class FlashSWDAWithSinkVarlen(torch.autograd.Function):
 def flash_swda_with_sink_varlen(q, k, v, cu_seqlens: CuSeqlens, window_size: int,
                                 sink_size: int = 0, is_causal: bool = True,
                                 scale: Optional[float] = None,
-                                sinks: Optional[torch.Tensor] = None):
+                                sinks: Optional[torch.Tensor] = None, rotary=None,
+                                positions: Optional[torch.Tensor] = None):
     """``flash_swda_with_sink`` over packed sequences: q ``[T, Hq, D]``, k, v ``[T, Hkv, D]``,
-    ``cu_seqlens`` ``batch + 1`` offsets; returns o ``[T, Hq, D]``."""
+    ``cu_seqlens`` ``batch + 1`` offsets; returns o ``[T, Hq, D]``.  ``rotary`` with
+    ``positions`` (``[T]`` or ``[axes, T]``): q and k are rotated first."""
+    q, k = rotated(q, k, rotary, positions)
     return FlashSWDAWithSinkVarlen.apply(q, k, v, cu_seqlens, window_size, sink_size, is_causal,
                                          scale, sinks)

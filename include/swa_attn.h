@@ -54,7 +54,8 @@ typedef enum SwaStatus {
   SWA_ERR_LAUNCH = 3,        /* the CUDA launch itself failed (see swa_last_cuda_error) */
   SWA_ERR_DEVICE_TIMEOUT = 4,/* a bounded on-device wait gave up                        */
   SWA_ERR_WORKSPACE = 5,     /* workspace missing or smaller than swa_bwd_workspace_size */
-  SWA_ERR_TOO_LARGE = 6      /* problem needs more scratch than swa_bwd_no_alloc holds   */
+  SWA_ERR_TOO_LARGE = 6,     /* problem needs more scratch than swa_bwd_no_alloc holds   */
+  SWA_ERR_BAD_PAGE = 7       /* a page table entry or a length was out of range          */
 } SwaStatus;
 
 typedef enum SwaDtype { SWA_F16 = 0, SWA_BF16 = 1 } SwaDtype;
@@ -201,6 +202,131 @@ SWA_API int swa_varlen_fwd(const SwaVarlenFwdArgs* args, void* stream);
  * dsink_logits sums the sequences' contributions in sequence order). */
 SWA_API int swa_varlen_bwd(const SwaVarlenBwdArgs* args, void* stream);
 
+/* ------------------------------------------------------------------------------------
+ * Rotary positions (an additional operator with no counterpart in the reference, which takes
+ * q and k as they are).  Frequency i of n_freq turns one pair of a head's values by the angle
+ * theta_i = position[axis[i]] * inv_freq[i]:
+ *   (x, y) -> scale * (x cos theta_i - y sin theta_i, y cos theta_i + x sin theta_i),
+ * where the pair is (i, n_freq + i), or (2 i, 2 i + 1) with `interleaved`; values from
+ * 2 n_freq on are copied.  A token has one position per axis (time, height, width for images
+ * and video; one axis for text).  With `inverse` the angle is negated: the gradient of the
+ * inputs from the gradient of the outputs.  Angles are formed in 64 bits, products and sums in
+ * 32, one rounding to the tensors' type at the end.
+ * ------------------------------------------------------------------------------------ */
+#define SWA_ROTARY_MAX_FREQS 64
+
+typedef struct SwaRotary {
+  const float* inv_freq;       /* device, n_freq values                                   */
+  const void* positions;       /* device, int32 or int64: positions[axis, b, l]           */
+  int64_t pos_stride_axis, pos_stride_b, pos_stride_l; /* in elements; 0 broadcasts       */
+  int32_t pos_is_64;           /* 1: positions are int64                                  */
+  int32_t n_axes;              /* >= 1                                                    */
+  int32_t n_freq;              /* 0 .. 64, 2 n_freq <= head_dim                           */
+  int32_t interleaved;
+  float scale;
+  uint8_t axis[SWA_ROTARY_MAX_FREQS]; /* axis of each frequency, < n_axes                 */
+} SwaRotary;
+
+typedef struct SwaRotaryArgs {
+  int32_t batch, n_q_heads, n_kv_heads, seq_len, head_dim; /* head_dim even, <= 128       */
+  int32_t dtype;               /* SwaDtype                                                */
+  int32_t inverse;
+  SwaRotary r;
+  SwaTensor q, k;              /* [B, Hq, L, D], [B, Hkv, L, D]; k.ptr NULL: q alone       */
+  SwaTensor q_out, k_out;      /* may be the inputs themselves (same pointer and strides)  */
+} SwaRotaryArgs;
+
+/* Rotate q and k.  Any strides >= 0 (rows need not be 16-byte aligned; aligned ones are read
+ * and written 16 bytes at a time).  Outputs must not overlap inputs unless they are them. */
+SWA_API int swa_rotary(const SwaRotaryArgs* args, void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * Paged key-value cache (additional operators with no counterpart in the reference, which
+ * trains only).  Keys and values of a sequence lie in pages of page_size rows from one pool;
+ * slot j of sequence b is row j % page_size of page page_table[b, j / page_size].  seq_lens[b]
+ * slots are in use.  All integer arrays are DEVICE arrays: no call reads them on the host.
+ * Table entries behind a sequence's last page are not read.  An entry outside [0, n_pages) or
+ * a length above max_pages * page_size that a call meets is never followed: rows of such pages
+ * are neither read nor written, the sequence's attention output is NaN, and a following
+ * swa_check_device returns SWA_ERR_BAD_PAGE.  A negative length counts as 0.
+ * ------------------------------------------------------------------------------------ */
+typedef struct SwaPagedKV {
+  void* k;                     /* [n_pages, n_kv_heads, page_size, D], D contiguous        */
+  void* v;
+  int64_t k_stride_page, k_stride_head, k_stride_row; /* elements, multiples of 8          */
+  int64_t v_stride_page, v_stride_head, v_stride_row;
+  const int32_t* page_table;   /* [batch, max_pages], row stride table_stride              */
+  int64_t table_stride;
+  int32_t* seq_lens;           /* [batch]; written by swa_paged_evict alone                */
+  const int32_t* seen;         /* [batch] tokens seen so far, or NULL: seq_lens            */
+  float* weights;              /* [batch, n_kv_heads, max_pages * page_size], or NULL      */
+  int32_t* positions;          /* same shape: the token number of each slot, or NULL       */
+  int64_t w_stride_b, w_stride_h, p_stride_b, p_stride_h; /* elements                      */
+  int32_t n_pages, page_size, max_pages; /* page_size: a multiple of 16                    */
+  int32_t batch, n_kv_heads, head_dim, dtype; /* head_dim 16, 32, 64 or 128               */
+} SwaPagedKV;
+
+typedef struct SwaPagedAppendArgs {
+  SwaPagedKV cache;            /* seq_lens (and seen) already count the new tokens         */
+  const int32_t* cu_new;       /* device, batch + 1 offsets of the packed new tokens, or
+                                  NULL: n_tokens / batch tokens for every sequence         */
+  int32_t n_tokens;
+  int32_t n_q_heads;           /* 0: no q                                                  */
+  SwaPackedTensor k, v;        /* new tokens, [n_tokens, n_kv_heads, D]                    */
+  SwaPackedTensor q, q_out;    /* [n_tokens, n_q_heads, D]: rotated beside k               */
+  int32_t use_rotary;          /* 0: k is written as it is (and q must be absent)          */
+  SwaRotary r;                 /* positions[axis, 0, token]                                */
+} SwaPagedAppendArgs;
+
+/* Write new tokens into the cache, rotating k (and q) on the way.  Token i of sequence b goes
+ * to slot seq_lens[b] - new_b + i; its weight becomes 0 and its position the token number
+ * seen[b] - new_b + i (where those arrays are given). */
+SWA_API int swa_paged_append(const SwaPagedAppendArgs* args, void* stream);
+
+typedef struct SwaPagedDecodeArgs {
+  SwaPagedKV cache;
+  int32_t n_q_heads;           /* Hq, a multiple of n_kv_heads                             */
+  int32_t window_size, sink_size; /* over slots, the newest token at slot seq_lens[b] - 1  */
+  float softmax_scale;
+  SwaPackedTensor q, o;        /* [batch, n_q_heads, D]; stride_t is the batch stride      */
+  float* lse;                  /* [batch, n_q_heads] contiguous fp32, or NULL              */
+  const float* sink_logits;    /* [n_q_heads] fp32 or NULL (see swa_fwd_sink_logits)       */
+  float* weights_out;          /* NULL, or like cache.weights (may be it): see below       */
+  int64_t wo_stride_b, wo_stride_h;
+  float decay;
+  void* workspace;             /* >= swa_paged_decode_workspace_size bytes, 256-B aligned  */
+  size_t workspace_bytes;
+} SwaPagedDecodeArgs;
+
+/* Attention of one new token per sequence over its cache: slot j < n = seq_lens[b] is visible
+ * iff n - 1 - j < window_size or j < sink_size.  lse as in swa_fwd.  With weights_out:
+ *   weights_out[b, h, j] = decay * cache.weights[b, h, j] + sum over the query heads of KV
+ * head h of their softmax weight on slot j (0 where it is not visible), for j < n. */
+SWA_API int swa_paged_decode(const SwaPagedDecodeArgs* args, void* stream);
+
+/* Scratch that swa_paged_decode needs (pointers are not looked at, except weights_out for
+ * NULL). */
+SWA_API size_t swa_paged_decode_workspace_size(const SwaPagedDecodeArgs* args);
+
+typedef struct SwaPagedEvictArgs {
+  SwaPagedKV cache;            /* weights and positions given                              */
+  int32_t keep;                /* slots left to a sequence that is cut                     */
+  int32_t trigger;             /* sequences with more slots than max(trigger, keep) are cut */
+  int32_t sink_size;           /* tokens numbered below it are held ...                    */
+  int32_t recent;              /* ... and those from seen[b] - recent on                   */
+  void* workspace;             /* >= swa_paged_evict_workspace_size bytes, 256-B aligned   */
+  size_t workspace_bytes;
+} SwaPagedEvictArgs;
+
+/* Cut every sequence longer than max(trigger, keep) down to keep slots, each KV head by its own
+ * weights: held tokens stay first, then those of the largest weights (ties: the lowest slot;
+ * NaN counts as -inf).  A kept slot below `keep` stays where it is; the i-th slot that comes
+ * free below `keep` takes key, value, weight and position of the i-th kept slot from `keep` on,
+ * and seq_lens[b] becomes keep.  Pages of a sequence that is cut must not belong to another
+ * sequence too. */
+SWA_API int swa_paged_evict(const SwaPagedEvictArgs* args, void* stream);
+SWA_API size_t swa_paged_evict_workspace_size(const SwaPagedEvictArgs* args);
+
 /* Backward that allocates nothing and takes no workspace.  No counterpart in the reference.
  *
  * For callers that cannot call cudaMalloc: a host that hands this library only its tensors
@@ -223,7 +349,8 @@ SWA_API int swa_bwd_no_alloc(const SwaBwdArgs* args, void* stream);
  *
  * Synchronise `stream`, then report (and clear) the current device's on-device error flag:
  * SWA_ERR_DEVICE_TIMEOUT if a bounded wait inside a kernel gave up since the last check
- * (that launch's outputs are then undefined), SWA_OK otherwise. */
+ * (that launch's outputs are then undefined), SWA_ERR_BAD_PAGE if a paged call met a page or a
+ * length out of range, SWA_OK otherwise. */
 SWA_API int swa_check_device(void* stream);
 
 /* Enqueue on `stream` a copy of the current device's on-device error flag into

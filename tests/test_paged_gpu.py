@@ -1,0 +1,536 @@
+"""GPU parity of the paged-cache operators (append, single-token attention, eviction) against the
+64-bit oracle, through the public API.
+
+The pool starts as NaN everywhere: only the slots that a call may read are filled, so a read of
+any other row (behind a sequence, outside the window, on a page of nobody) shows as NaN.
+
+Tolerances of the attention, derived, with delta = max_j sum_d |q_d k_jd| scale for a row and
+A = sum_j p_j |v_j|: a 32-bit score of D products, added one after the other, is off by at most
+(D + 2) 2^-24 delta; a weight exp(s - m) by twice that (its own score's and the maximum's are the
+same sums, the row sum adds another) and 2^-21 for exp2 and its argument's rounding; a weight that
+is multiplied in 16-bit pieces by 2^-16 at most (two pieces of bf16: 2^-9 2^-9 = 2^-18, twice);
+the sums over n slots add n/8 2^-23 (no element is added to more than n / 16 + 32 partial sums,
+tensor cores cut instead of rounding, and once more for the row sum).  Then the output is rounded
+once (eps / 2 of the value, for fp16 at least 2^-25).
+"""
+import math
+
+import pytest
+import torch
+
+from oracle import serving_oracle as orc
+from tests._pkg import pkg, submodule
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+WHOLE = 2**31 - 1
+
+
+def relative(d, n, delta):
+    """Bound on the relative error of a row's weights."""
+    return 4 * (d + 2) * 2.0**-24 * delta + 2.0**-20 + 2.0**-16 + (n / 8 + 64) * 2.0**-23
+
+
+class Case:
+    """A cache on the GPU and, per sequence, the dense rows [Hkv, n, D] that it holds (on the CPU)."""
+
+    def __init__(self, lens, hkv=2, d=64, page=16, dtype=torch.bfloat16, seed=0, extra=2, track=False, room=0,
+                 rows_first=False, live=None, scale=1.0):
+        g = torch.Generator().manual_seed(seed)
+        self.g, self.lens, self.dtype, self.page = g, list(lens), dtype, page
+        b = len(lens)
+        m = max(1, max((-(-(n + room) // page) for n in lens), default=1))
+        n_pages = b * m + extra
+        perm = torch.randperm(n_pages, generator=g)
+        table = torch.full((b, m), -1, dtype=torch.int32)
+        shape = (n_pages, page, hkv, d) if rows_first else (n_pages, hkv, page, d)
+        pools = [torch.full(shape, math.nan, dtype=dtype) for _ in range(2)]
+        if rows_first:  # pages of [rows, heads, D], seen as [heads, rows, D]
+            pools = [x.transpose(1, 2) for x in pools]
+        self.rows = []
+        for i, n in enumerate(lens):
+            used = -(-(n + room) // page)
+            table[i, :used] = perm[i * m:i * m + used].to(torch.int32)
+            kv = []
+            for x in pools:
+                r = (torch.randn(hkv, n, d, generator=g) * scale).to(dtype)
+                for j in (range(n) if live is None else live(n)):
+                    x[table[i, j // page], :, j % page] = r[:, j]
+                kv.append(r)
+            self.rows.append(kv)
+        self.cap = m * page
+        self.k, self.v = (x.to(DEV) for x in pools)
+        assert self.k.stride() == pools[0].stride()
+        self.table = table.to(DEV)
+        self.lens_t = torch.tensor(self.lens, dtype=torch.int32, device=DEV)
+        kw = {}
+        if track:
+            kw = dict(weights=torch.rand(b, hkv, self.cap, generator=g).to(DEV),
+                      positions=torch.arange(self.cap, dtype=torch.int32).expand(b, hkv, self.cap).contiguous().to(DEV),
+                      seen=self.lens_t.clone())
+        self.cache = pkg().PagedKVCache(self.k, self.v, self.table, self.lens_t, **kw)
+
+
+def check_decode(c, q, window=None, sinks=0, logits=None, scale=None, weights=None, decay=1.0, old=None):
+    """Run and compare every output; ``weights``: weights_out, with ``old`` the weights before."""
+    qd = q if q.is_cuda else q.to(DEV)
+    before = None if weights is None else weights.cpu().clone()
+    o, lse = c.cache.decode(qd, window_size=window, sink_size=sinks, sinks=None if logits is None else logits.to(DEV),
+                            softmax_scale=scale, weights_out=weights, decay=decay, return_lse=True)
+    c.cache.check()
+    assert o.shape == q.shape and o.dtype == q.dtype
+    o, lse = o.double().cpu(), lse.double().cpu()
+    d, hkv = q.shape[2], c.k.shape[1]
+    g = q.shape[1] // hkv
+    eps = torch.finfo(q.dtype).eps / 2
+    floor = 2.0**-25 if q.dtype == torch.float16 else 0.0
+    for i, n in enumerate(c.lens):
+        ro, rl, p, amount, delta = orc.decode(q[i], *c.rows[i], n, WHOLE if window is None else window, sinks, scale, logits)
+        rel = relative(d, n, delta)
+        wide = rel[:, None] * amount
+        err = (o[i] - ro).abs()
+        assert bool((err <= (eps * (ro.abs() + wide)).clamp_min(floor) + wide).all()), (i, n, float(err.max()))
+        same = torch.isinf(rl)
+        assert bool((lse[i][same] == rl[same]).all()), (i, n)
+        # lse in base 2: the row sum's relative error over ln 2, and the 32-bit value's own half step
+        lim = rel / math.log(2) + 2.0**-22 * (1 + rl.abs())
+        assert bool(((lse[i] - rl).abs()[~same] <= lim[~same]).all()), (i, n)
+        if weights is not None:
+            w = weights[i].double().cpu()
+            add = p.view(hkv, g, n).sum(1)
+            was = torch.zeros(hkv, n).double() if old is None else old[i, :, :n].double().cpu()
+            ref = decay * was + add
+            lim = add * rel.view(hkv, g).amax(1)[:, None] + 2.0**-22 * (ref.abs() + (decay * was).abs() + add) + 1e-37
+            assert bool(((w[:, :n] - ref).abs() <= lim).all()), (i, n)
+            assert torch.equal(w[:, n:], before[i, :, n:].double())  # slots behind the sequence: left alone
+
+
+def queries(c, hq, d, mult=2.0):
+    return (torch.randn(len(c.lens), hq, d, generator=c.g) * mult).to(c.dtype)
+
+
+LENS = [0, 1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 129, 300]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+@pytest.mark.parametrize("hq,hkv", [(8, 8), (16, 2), (6, 2), (40, 2)], ids=["g1", "g8", "g3", "g20"])
+def test_decode_whole_cache(dtype, d, hq, hkv):
+    c = Case(LENS, hkv, d, 16, dtype, seed=d + hq)
+    check_decode(c, queries(c, hq, d))
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (0, 3), (1, 0), (5, 20), (16, 0), (64, 4), (100, 16), (128, 300), (1000, 4)])
+@pytest.mark.parametrize("page", [16, 48, 128])
+def test_decode_windows_and_sinks(window, sinks, page):
+    live = lambda n: orc.visible(n, window, sinks)  # noqa: E731
+    c = Case(LENS + [700], 2, 64, page, seed=window + sinks, live=live)
+    check_decode(c, queries(c, 16, 64), window, sinks)
+    logits = torch.randn(16, generator=c.g) * 3
+    logits[3], logits[5] = -math.inf, 50.0
+    check_decode(c, queries(c, 16, 64), window, sinks, logits=logits)
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(16, 2, 64, torch.bfloat16), (12, 1, 128, torch.float16), (4, 4, 16, torch.float16),
+                                            (40, 2, 32, torch.bfloat16)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (70, 5)])
+def test_decode_weights(hq, hkv, d, dtype, window, sinks):
+    live = None if window is None else lambda n: orc.visible(n, window, sinks)  # noqa: E731
+    c = Case(LENS + [1100], hkv, d, 16, dtype, seed=hq, track=True, live=live)
+    out = torch.full_like(c.cache.weights, 7.0)
+    old = c.cache.weights.cpu().clone()
+    logits = torch.randn(hq, generator=c.g)
+    check_decode(c, queries(c, hq, d), window, sinks, logits=logits, weights=out, decay=0.5, old=old)
+    assert torch.equal(c.cache.weights.cpu(), old)
+    check_decode(c, queries(c, hq, d), window, sinks, weights=c.cache.weights, old=old)  # in place
+    bare = pkg().PagedKVCache(c.k, c.v, c.table, c.lens_t)
+    c.cache = bare
+    check_decode(c, queries(c, hq, d), window, sinks, weights=out)  # no weights of before: the new ones alone
+
+
+@pytest.mark.parametrize("lens,hq,hkv,d", [([20000], 8, 1, 64), ([5000, 3, 0, 9000], 16, 2, 128), ([30000, 1], 4, 4, 16),
+                                           ([4096] * 3 + [17] * 30, 8, 2, 64), ([70000], 64, 8, 32)])
+def test_decode_long_and_ragged(lens, hq, hkv, d):
+    c = Case(lens, hkv, d, 64, seed=lens[0], track=True)
+    out = torch.zeros_like(c.cache.weights)
+    check_decode(c, queries(c, hq, d, 4.0), weights=out, old=c.cache.weights.cpu())
+    check_decode(c, queries(c, hq, d, 4.0), window=3000, sinks=7)
+
+
+def test_decode_many_sequences():
+    lens = [(37 * i) % 211 for i in range(700)]
+    c = Case(lens, 1, 32, 32, torch.float16, seed=1)
+    check_decode(c, queries(c, 4, 32))
+    check_decode(c, queries(c, 4, 32), window=20, sinks=2)
+
+
+def test_decode_extreme_scores():
+    # scores of +-thousands: one key takes all; equal scores; a scale of 0 and a negative one
+    c = Case([200, 33], 2, 64, 16, torch.float16, seed=3, scale=8.0)
+    q = queries(c, 8, 64, 30.0)
+    check_decode(c, q)
+    check_decode(c, q, scale=0.0)
+    check_decode(c, q, scale=-0.125)
+    c.rows = [[k[:, :1].expand_as(k).clone(), v] for k, v in c.rows]
+    for i, (k, _) in enumerate(c.rows):
+        for j in range(c.lens[i]):
+            c.k[c.table[i, j // 16], :, j % 16] = k[:, j].to(DEV)
+    check_decode(c, q)
+
+
+def test_decode_strides():
+    # pages of [rows, heads, D]; q from one projection with k and v; tables with a longer row
+    c = Case([100, 257, 3], 4, 64, 48, seed=4, rows_first=True)
+    qkv = torch.randn(3, 24, 64, generator=c.g).bfloat16().to(DEV)
+    check_decode(c, qkv[:, :16].cpu().to(DEV)[:, :16])
+    o1 = c.cache.decode(qkv[:, 2:18])
+    o2 = c.cache.decode(qkv[:, 2:18].contiguous())
+    assert torch.equal(o1, o2)
+    odd = torch.empty(3 * 16 * 64 + 1, dtype=torch.bfloat16, device=DEV)[1:].view(3, 16, 64)
+    odd.copy_(qkv[:, 2:18])
+    assert torch.equal(c.cache.decode(odd), o2)
+    wide = torch.full((3, 50), 12345678, dtype=torch.int32, device=DEV)
+    wide[:, :c.table.shape[1]] = c.table
+    cache = pkg().PagedKVCache(c.k, c.v, wide[:, :c.table.shape[1]], c.lens_t)
+    assert torch.equal(cache.decode(qkv[:, 2:18]), o2)
+
+
+def test_decode_is_deterministic_and_shares_pages():
+    c = Case([3000, 500], 2, 64, 64, seed=5)
+    q = queries(c, 16, 64).to(DEV)
+    a = c.cache.decode(q)
+    assert all(torch.equal(a, c.cache.decode(q)) for _ in range(5))
+    # two sequences over the same pages, their weights apart
+    table = c.table[:1].expand(2, -1).contiguous()
+    lens = torch.tensor([3000, 2999], dtype=torch.int32, device=DEV)
+    cache = pkg().PagedKVCache(c.k, c.v, table, lens)
+    w = torch.zeros(2, 2, c.cap, device=DEV)
+    o = cache.decode(torch.stack([q[0], q[0]]), weights_out=w)
+    assert torch.equal(o[0], a[0])
+    assert abs(float(w[1].sum()) - 16) < 1e-3 and float(w[1, :, 2999:].sum()) == 0
+
+
+def test_long_offsets():
+    # a pool whose rows lie beyond 2^31 elements
+    n_pages, page, hkv, d = 70000, 128, 2, 128
+    k = torch.empty(n_pages, hkv, page, d, dtype=torch.float16, device=DEV)
+    v = torch.empty_like(k)
+    assert k.numel() > 2**31
+    table = torch.tensor([[n_pages - 1, 3, n_pages - 2]], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([300], dtype=torch.int32, device=DEV)
+    w = torch.zeros(1, hkv, 384, device=DEV)
+    pos = torch.zeros(1, hkv, 384, dtype=torch.int32, device=DEV)
+    cache = pkg().PagedKVCache(k, v, table, lens, weights=w, positions=pos)
+    g = torch.Generator().manual_seed(6)
+    kn, vn = (torch.randn(300, hkv, d, generator=g).half() for _ in range(2))
+    cache.append(kn.to(DEV), vn.to(DEV))
+    c = Case.__new__(Case)
+    c.lens, c.dtype, c.g, c.cache, c.k = [300], torch.float16, g, cache, k
+    c.rows = [[kn.transpose(0, 1), vn.transpose(0, 1)]]
+    check_decode(c, queries(c, 8, d), weights=w, old=w.cpu().clone())
+    cache.evict(200)
+    cache.check()
+    assert lens.item() == 200 and torch.isfinite(cache.decode(queries(c, 8, d).to(DEV))).all()
+
+
+@pytest.mark.parametrize("even", [True, False])
+@pytest.mark.parametrize("hq,hkv,d,page,dtype", [(8, 2, 64, 16, torch.bfloat16), (4, 4, 128, 48, torch.float16), (6, 1, 16, 64, torch.float16)])
+def test_append(even, hq, hkv, d, page, dtype):
+    old = [0, 5, 16, 47, 48]
+    new = [3] * 5 if even else [0, 1, 33, 2, 70]
+    c = Case(old, hkv, d, page, dtype, seed=7, track=True, room=80)
+    c.cache.seen.add_(1000)  # an eviction has left fewer slots than tokens
+    t = sum(new)
+    q, k, v = (torch.randn(t, h, d, generator=c.g).to(dtype) for h in (hq, hkv, hkv))
+    n = d // 2
+    inv = (1000.0 ** (-torch.arange(n) / n)).float()
+    sections = (n - 4, 2, 2)
+    axes = [a for a, x in enumerate(sections) for _ in range(x)]
+    rot = pkg().Rotary(inv.to(DEV), sections=sections, scale=1.5)
+    pos = torch.randint(0, 100000, (3, t), generator=c.g)
+    bits = torch.int16
+    before = [x.cpu().view(bits) for x in (c.k, c.v)]
+    w0, p0 = c.cache.weights.cpu(), c.cache.positions.cpu()
+    c.cache.advance(torch.tensor(new, dtype=torch.int32, device=DEV))
+    cu = None if even else torch.tensor([0] + new).cumsum(0).to(torch.int32).to(DEV)
+    yq = c.cache.append(k.to(DEV), v.to(DEV), cu_new=cu, q=q.to(DEV), positions=pos.to(DEV), rotary=rot)
+    c.cache.check()
+    rq, rk = (submodule("rotary").rotate(x.to(DEV), None, pos.to(DEV), rot)[0] for x in (q, k))
+    # the same arithmetic as the rotation alone, which has its own tests
+    assert torch.equal(yq, rq)
+    at = 0
+    table = c.table.cpu()
+    expect = [x.clone() for x in before]
+    for i, (a, m) in enumerate(zip(old, new)):
+        for j in range(m):
+            slot = a + j
+            page_i, row = table[i, slot // page], slot % page
+            expect[0][page_i, :, row] = rk[at].cpu().view(bits)
+            expect[1][page_i, :, row] = v[at].view(bits)
+            w0[i, :, slot], p0[i, :, slot] = 0.0, slot + 1000
+            at += 1
+    for x, y in zip((c.k, c.v), expect):
+        assert torch.equal(x.cpu().view(bits), y)  # new rows, and nothing else
+    assert torch.equal(c.cache.weights.cpu(), w0) and torch.equal(c.cache.positions.cpu(), p0)
+    check(rk, k, pos, inv, axes, 1.5)
+
+
+def check(y, x, pos, inv, axes, scale):
+    from tests.test_rotary_gpu import check as same
+    same(x.transpose(0, 1), y.transpose(0, 1), pos[:, None], inv, axes, False, scale)
+
+
+def test_append_without_rotation_and_strides():
+    c = Case([40, 0], 2, 64, 16, seed=8, room=30, rows_first=True)
+    kv = torch.randn(2, 20, 4, 64, generator=c.g).bfloat16()
+    flat = kv.to(DEV).view(40, 4, 64)
+    c.cache.advance(20)
+    assert c.cache.append(flat[:, :2], flat[:, 2:]) is None
+    c.rows = [[torch.cat([o, kv[i, :, 2 * s:2 * s + 2].transpose(0, 1)], 1) for s, o in enumerate(c.rows[i])] for i in range(2)]
+    c.lens = [60, 20]
+    check_decode(c, queries(c, 8, 64))
+
+
+@pytest.mark.parametrize("values", ["spread", "ties", "zeros", "odd"])
+@pytest.mark.parametrize("keep,trigger,sinks,recent", [(1, None, 0, 0), (32, None, 4, 8), (64, 80, 0, 64), (100, None, 100, 0), (299, None, 3, 20)])
+def test_evict(values, keep, trigger, sinks, recent):
+    lens = [0, 1, 31, 32, 33, 64, 65, 81, 300, 300, 1]
+    c = Case(lens, 3, 32, 16, torch.float16, seed=keep, track=True)
+    b, h, cap = len(lens), 3, c.cap
+    w = {"spread": lambda: torch.exp(3 * torch.randn(b, h, cap, generator=c.g)),
+         "ties": lambda: torch.randint(0, 3, (b, h, cap), generator=c.g).float(),
+         "zeros": lambda: torch.zeros(b, h, cap) * torch.where(torch.rand(b, h, cap, generator=c.g) < 0.5, 1.0, -1.0),
+         "odd": lambda: torch.tensor([math.nan, math.inf, -math.inf, -1.0, 0.0, -0.0, 1e-42, -1e-42, 3e38])[
+             torch.randint(0, 9, (b, h, cap), generator=c.g)]}[values]()
+    c.cache.weights.copy_(w)
+    order = torch.stack([torch.randperm(cap, generator=c.g) for _ in range(b * h)]).view(b, h, cap).to(torch.int32)
+    c.cache.positions.copy_(order)
+    seen = torch.tensor([cap + 5] * b, dtype=torch.int32)
+    c.cache.seen.copy_(seen)
+    k, v, w, pos = (x.cpu().clone() for x in (c.k, c.v, c.cache.weights, c.cache.positions))
+    bits = lambda x: x.view(torch.int16 if x.dtype == torch.float16 else torch.int32)  # noqa: E731
+    k, v, w = bits(k), bits(v), bits(w)
+    before = [x.clone() for x in (k, v, w, pos)]
+    c.cache.evict(keep, sinks, recent, trigger)
+    c.cache.check()
+    table = c.table.cpu()
+    new = []
+    for i, n in enumerate(lens):
+        cut = n > max(keep, trigger or 0)
+        new.append(keep if cut else n)
+        if not cut:
+            continue
+        for x in range(h):
+            free, movers = orc.evict(before[2][i, x].view(torch.float32), before[3][i, x], n, int(seen[i]), keep, sinks, recent)
+            assert len(free) == len(movers)
+            for to, fr in zip(free, movers):
+                for pool, old in ((k, before[0]), (v, before[1])):
+                    pool[table[i, to // 16], x, to % 16] = old[table[i, fr // 16], x, fr % 16]
+                w[i, x, to], pos[i, x, to] = before[2][i, x, fr], before[3][i, x, fr]
+    assert c.lens_t.tolist() == new
+    for got, ref in ((bits(c.k), k), (bits(c.v), v), (bits(c.cache.weights), w), (c.cache.positions, pos)):
+        assert torch.equal(got.cpu(), ref)
+
+
+@pytest.mark.parametrize("n,keep,hkv,b", [(20000, 3000, 2, 1), (9000, 8999, 1, 2), (5000, 1, 1, 1), (2049, 1024, 8, 3), (120000, 17000, 1, 1)])
+def test_evict_long(n, keep, hkv, b):
+    d, page = 16, 64
+    lens = [n - 7 * i for i in range(b)]
+    m = -(-n // page)
+    g = torch.Generator().manual_seed(n)
+    k, v = (torch.randn(b * m, hkv, page, d, generator=g).half().to(DEV) for _ in range(2))
+    table = torch.randperm(b * m, generator=g).view(b, m).to(torch.int32)
+    w = torch.exp(3 * torch.randn(b, hkv, m * page, generator=g))
+    w[torch.rand(w.shape, generator=g) < 0.3] = 0.0
+    pos = torch.arange(m * page, dtype=torch.int32).expand(w.shape).contiguous()
+    wd, pd, lt = w.to(DEV), pos.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    cache = pkg().PagedKVCache(k, v, table.to(DEV), lt, weights=wd, positions=pd)
+    k0, v0 = k.cpu(), v.cpu()
+    recent = min(keep - 1, 64) if keep > 1 else 0
+    cache.evict(keep, sink_size=min(1, keep - recent), recent=recent)
+    cache.check()
+    assert lt.tolist() == [min(ln, keep) for ln in lens]
+    k1, v1, w1, p1 = k.cpu(), v.cpu(), wd.cpu(), pd.cpu()
+    for i, ln in enumerate(lens):
+        for x in range(hkv):
+            cut = ln > keep
+            free, movers = orc.evict(w[i, x], pos[i, x], ln, ln, keep, min(1, keep - recent), recent) if cut else ([], [])
+            to, fr = torch.tensor(free, dtype=torch.long), torch.tensor(movers, dtype=torch.long)
+            ew, ep = w[i, x].clone(), pos[i, x].clone()
+            ew[to], ep[to] = w[i, x][fr], pos[i, x][fr]
+            assert torch.equal(w1[i, x], ew) and torch.equal(p1[i, x], ep)
+            for a, z in ((k0, k1), (v0, v1)):
+                rows = a[table[i].long(), x].reshape(-1, d).clone()
+                rows[to] = rows[fr].clone()
+                assert torch.equal(z[table[i].long(), x].reshape(-1, d), rows)
+
+
+def test_bad_pages_and_lengths_are_not_followed():
+    L = submodule("_lib")
+    c = Case([200, 40, 100, 60], 2, 64, 16, seed=9, track=True, room=4)
+    q = queries(c, 8, 64)
+    good = c.cache.decode(q.to(DEV))
+    c.cache.check()
+    c.table[0, 5] = c.k.shape[0]      # just past the pool
+    c.table[1, 1] = -1
+    c.lens_t[2] = c.cap + 1           # more than the table holds
+    w = torch.zeros_like(c.cache.weights)
+    for kw in ({}, {"weights_out": w}):
+        o = c.cache.decode(q.to(DEV), **kw)
+        with pytest.raises(L.SwaError) as e:
+            c.cache.check()
+        assert e.value.status == L.SWA_ERR_BAD_PAGE
+        assert torch.isnan(o[:3].float()).all() and torch.equal(o[3], good[3])
+        c.cache.check()               # reported once
+    k = c.k.cpu().view(torch.int16).clone()
+    # appends behind bad ends: the good sequence alone is written
+    c.lens_t.copy_(torch.tensor([96, 32, c.cap + 1, 61], dtype=torch.int32))
+    new = torch.randn(4, 2, 64, generator=c.g).bfloat16().to(DEV)
+    c.table[0, 5], c.table[1, 1] = -7, 2**31 - 1
+    c.cache.append(new, new)
+    with pytest.raises(L.SwaError):
+        c.cache.check()
+    k[c.table[3, 3].item(), :, 12] = new[3].cpu().view(torch.int16)
+    assert torch.equal(c.k.cpu().view(torch.int16), k)
+    # more new tokens than slots
+    c.lens_t.copy_(torch.tensor([0, 0, -5, 0], dtype=torch.int32))
+    c.cache.append(new, new)
+    with pytest.raises(L.SwaError):
+        c.cache.check()
+    assert torch.equal(c.k.cpu().view(torch.int16), k)
+    # an eviction moves what it can reach, and never a length out of range
+    c.lens_t.copy_(torch.tensor([90, 90, c.cap + 1, 60], dtype=torch.int32))
+    c.cache.evict(50)
+    with pytest.raises(L.SwaError):
+        c.cache.check()
+    assert c.lens_t.tolist()[2:] == [c.cap + 1, 50]
+
+
+def test_streams_and_graphs():
+    c = Case([300, 64, 1], 2, 64, 16, seed=10, track=True, room=200)
+    q = queries(c, 16, 64).to(DEV)
+    ref = c.cache.decode(q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = [c.cache.decode(q, weights_out=torch.zeros_like(c.cache.weights)) for _ in range(3)]
+    side.synchronize()
+    assert all(torch.equal(x, ref) for x in out)
+    # a step captured twice, replayed in turn with eager calls of the same cache
+    rot = pkg().Rotary((10000.0 ** (-torch.arange(32) / 32)).to(DEV))
+    k, v = (torch.randn(3, 2, 64, generator=c.g).bfloat16().to(DEV) for _ in range(2))
+    pos = torch.tensor([301, 65, 2], device=DEV)
+
+    def step():
+        c.cache.advance()
+        y = c.cache.append(k, v, q=q, positions=pos, rotary=rot)
+        return c.cache.decode(y, sink_size=4, weights_out=c.cache.weights)
+
+    state = [c.k, c.v, c.cache.weights, c.cache.positions, c.lens_t, c.cache.seen]
+    start = [x.clone() for x in state]
+
+    def back():
+        for x, y in zip(state, start):
+            x.copy_(y)
+
+    want = []
+    for _ in range(6):
+        want.append(step().clone())
+    end = [x.clone() for x in state]
+    back()
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step())
+        graphs.append(graph)
+    back()
+    got = []
+    for i in range(6):
+        if i % 3 == 2:
+            got.append(step().clone())
+        else:
+            graphs[i % 3].replay()
+            got.append(outs[i % 3].clone())
+    for x, y in zip(got + state, want + end):
+        assert torch.equal(x.nan_to_num(), y.nan_to_num())
+
+
+def test_serving_run():
+    """Prompts in, tokens out, evictions between: against the 64-bit oracle, slot by slot."""
+    hq, hkv, d, page, keep, sinks, recent = 8, 2, 32, 16, 40, 2, 10
+    cache = pkg().PagedKVCache.allocate(3, hkv, d, 160, page, torch.float16, DEV, track=True)
+    g = torch.Generator().manual_seed(11)
+    inv = (10000.0 ** (-torch.arange(16) / 16)).float()
+    rot = pkg().Rotary(inv.to(DEV))
+    axes, logits = [0] * 16, torch.randn(hq, generator=g)
+    prompt = [70, 5, 39]
+    held = [[dict(k=torch.zeros(0, d), v=torch.zeros(0, d), w=[], pos=[]) for _ in range(hkv)] for _ in prompt]
+    seen = [0, 0, 0]
+
+    def put(new, pos, k, v):
+        """The oracle's append, of the rows that the cache has written (their rotation is tested elsewhere)."""
+        at = 0
+        for i, m in enumerate(new):
+            for h in range(hkv):
+                s = held[i][h]
+                s["k"] = torch.cat([s["k"], k[at:at + m, h].double()])
+                s["v"] = torch.cat([s["v"], v[at:at + m, h].double()])
+                s["w"] += [0.0] * m
+                s["pos"] += list(range(seen[i], seen[i] + m))
+            seen[i] += m
+            at += m
+
+    def decode(q):
+        o = cache.decode(q, sinks=logits.to(DEV), weights_out=cache.weights)
+        cache.check()
+        for i in range(3):
+            n = len(held[i][0]["w"])
+            k, v = (torch.stack([held[i][h][x] for h in range(hkv)]) for x in "kv")
+            ro, _, p, amount, delta = orc.decode(q[i].cpu(), k, v, n, WHOLE, 0, None, logits)
+            rel = relative(d, n, delta)[:, None] * amount
+            err = (o[i].double().cpu() - ro).abs()
+            assert bool((err <= (2.0**-11 * (ro.abs() + rel)).clamp_min(2.0**-25) + rel).all())
+            for h in range(hkv):
+                add = p.view(hkv, -1, n)[h].sum(0).tolist()
+                held[i][h]["w"] = [a + b for a, b in zip(held[i][h]["w"], add)]
+            got = cache.weights[i, :, :n].double().cpu()
+            ref = torch.tensor([held[i][h]["w"] for h in range(hkv)], dtype=torch.float64)
+            # every step's weights carry the error above, and each sum half a step
+            assert bool(((got - ref).abs() <= ref * (relative(d, n, delta).max() + 40 * 2.0**-24) + 1e-12).all())
+            # go on with the cache's own weights, so that ties and near ties are decided alike
+            for h in range(hkv):
+                held[i][h]["w"] = cache.weights[i, h, :n].tolist()
+
+    def evict():
+        cache.evict(keep, sinks, recent)
+        cache.check()
+        for i in range(3):
+            n = len(held[i][0]["w"])
+            if n <= keep:
+                continue
+            for h in range(hkv):
+                s = held[i][h]
+                free, movers = orc.evict(s["w"], s["pos"], n, seen[i], keep, sinks, recent)
+                for to, fr in zip(free, movers):
+                    s["k"][to], s["v"][to], s["w"][to], s["pos"][to] = s["k"][fr], s["v"][fr], s["w"][fr], s["pos"][fr]
+                s["k"], s["v"], s["w"], s["pos"] = s["k"][:keep], s["v"][:keep], s["w"][:keep], s["pos"][:keep]
+            assert cache.positions[i, :, :keep].tolist() == [held[i][h]["pos"] for h in range(hkv)]
+        assert cache.seq_lens.tolist() == [len(x[0]["w"]) for x in held] and cache.seen.tolist() == seen
+
+    t = sum(prompt)
+    pos = torch.cat([torch.arange(m) for m in prompt])
+    k, v = (torch.randn(t, hkv, d, generator=g).half() for _ in range(2))
+    cache.advance(torch.tensor(prompt, dtype=torch.int32, device=DEV))
+    cu = torch.tensor([0] + prompt).cumsum(0).to(torch.int32).to(DEV)
+    cache.append(k.to(DEV), v.to(DEV), cu_new=cu, positions=pos.to(DEV), rotary=rot)
+    put(prompt, pos, submodule("rotary").rotate(k.to(DEV), None, pos.to(DEV), rot)[0].cpu(), v)
+    for step in range(45):
+        q, k, v = ((torch.randn(3, h, d, generator=g) * 2).half() for h in (hq, hkv, hkv))
+        pos = torch.tensor(seen)
+        cache.advance()
+        y = cache.append(k.to(DEV), v.to(DEV), q=q.to(DEV), positions=pos.to(DEV), rotary=rot)
+        put([1, 1, 1], pos, submodule("rotary").rotate(k.to(DEV), None, pos.to(DEV), rot)[0].cpu(), v)
+        decode(y)
+        if step % 4 == 3:
+            evict()
