@@ -138,7 +138,11 @@ int swa_paged_decode(const SwaPagedDecodeArgs* a, void* stream) {
   if (!packed_ok(a->q) || !packed_ok(a->o)) return SWA_ERR_INVALID_ARG;
   if (!aligned16(a->q.ptr) || a->q.stride_t % 8 || a->q.stride_h % 8) return SWA_ERR_UNSUPPORTED;
   if (!aligned16(a->o.ptr) || a->o.stride_t % 8 || a->o.stride_h % 8) return SWA_ERR_UNSUPPORTED;
-  if (a->weights_out && (a->wo_stride_b < 0 || a->wo_stride_h < 0)) return SWA_ERR_UNSUPPORTED;
+  if (a->weights_out) {
+    if (a->wo_stride_b < 0 || a->wo_stride_h < 0) return SWA_ERR_UNSUPPORTED;
+    // a thread per slot and KV head, 256 to a block
+    if (((int64_t)c.max_pages * c.page_size / 256 + 1) * c.n_kv_heads * c.batch > INT32_MAX) return SWA_ERR_UNSUPPORTED;
+  }
   if (int st = check_workspace(a->workspace, a->workspace_bytes, swa_paged_decode_workspace_size(a))) return st;
   if (int st = bind_flag(&c)) return st;
   return swa::host_record(swa::launch_paged_decode(c, *a, static_cast<cudaStream_t>(stream)));

@@ -1,137 +1,670 @@
-// swa_paged_decode.cu -- attention of one new token per sequence over its paged cache.
+// swa_paged_decode.cu -- attention of one new token per sequence over its paged cache, split over
+// the cache's length and joined.
 //
-// o[b, h] = softmax([scale q k_j (visible j), sink_h]) v.  One block per (query head, sequence):
-// each warp walks every fourth visible slot with a running maximum and sum, the four are joined
-// at the end.
+// o[b, h] = sum_j p_j v_j / l, p_j = exp2(s_j - m), s_j = scale log2(e) q k_j over the visible
+// slots j, with the running maximum m and sum l of an online softmax.  Partial (m, l, o) of
+// disjoint sets of slots are joined exactly: (m, l, o) -> (max m, sum l 2^(m - max), ...).
+//
+// Work is cut into units of 16 slots, all of one page.  The units of all sequences and KV heads,
+// in a row, are dealt out evenly to the warps of the grid, whatever the lengths: a warp walks its
+// range, a block joins its warps' pieces in shared memory, and a sequence that lies in one block
+// is finished there; one that spans blocks leaves a partial per block for join_kernel.  The
+// device alone knows the lengths, so the host needs none.  Where no sequence can have many
+// visible slots (a window), each (sequence, KV head) has a block of its own instead and nothing
+// is left to join.
+//
+// A warp keeps a ring of K and V units in shared memory filled by 16-byte cp.async.  It multiplies
+// with mma.sync m16n8k16: up to 8 (or 16) query heads of the KV head are the 16 rows, so K and V
+// are read once per group.  The operator is bound by the bytes of the cache: 8 heads of dim 64 need
+// 8 flops a byte.  (tcgen05 takes 64 or 128 rows and shared-memory operands, and a TMEM round trip
+// for the softmax of 8 rows; there is no rate to gain here.)  The weights p are multiplied as two
+// 16-bit pieces, hi + lo, so that rounding them adds 2^-18 (bf16) to a result that is rounded at
+// 2^-9: with 8 heads the lo pieces are the tile's other 8 rows and cost nothing.
+#include "sm100.cuh"
 #include "swa_host.cuh"
 #include "swa_paged.cuh"
 
 namespace swa {
 namespace {
 
-constexpr int kThreads = 128;
+using sm100::saddr;
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kUnit = 16;     // slots per unit
+constexpr int kSms = 148;
+constexpr int kJoinThreads = 128;
+constexpr int kWeightThreads = 256;
+
+template <int D> struct Shape {
+  static constexpr int kUnitBytes = 2 * kUnit * D * 2;  // K and V
+  static constexpr int kStages = D == 128 ? 3 : 4;
+  static constexpr int kRing = kStages * kUnitBytes;    // per warp
+  static constexpr int kBlocksPerSm = D == 128 ? 2 : 3;
+  static constexpr int kMaxBlocks = kSms * kBlocksPerSm;
+};
 
 struct DecodeParams {
   PagedParams c;
-  int Hq, W, S, D;
+  int Hq, G, tiles, W, S;  // tiles: row tiles per KV head
+  int units_per_page;
+  int max_units;           // bound on the units of a sequence
+  int whole;               // 1: a block per (sequence, KV head, tile)
   float scale_log2;
   const void* q; void* o;
   int64_t qb, qh, ob, oh;
-  float* lse;
+  float* lse;              // [B, Hq] or null
   const float* sinks;
   float* wout;
   int64_t wob, woh;
   float decay;
+  float* partials;         // [blocks][2] Partial
+  float* heads;            // [blocks][warps] Partial: the first piece of a warp that has two
+  float* scores;           // [B * Hkv * tiles][max_units][ROWS][16]
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) decode_kernel(DecodeParams p) {
-  const int h = blockIdx.x, b = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int hk = h / (p.Hq / p.c.n_kv_heads), D = p.D;
-  const T* q = static_cast<const T*>(p.q) + b * p.qb + h * p.qh;
-  bool bad = false;
-  const int n = paged_len(p.c, b, &bad);
-  const VisibleSlots vis = visible_slots(n, p.W, p.S);
-  const int total = vis.sinks + n - vis.first;
-  float m = -INFINITY, l = 0.f, acc[4] = {};
-  for (int u = warp; u < total; u += kThreads / 32) {
-    const int slot = u < vis.sinks ? u : u - vis.sinks + vis.first;
-    const int page = paged_page(p.c, b, slot / p.c.page_size, &bad);
-    if (page < 0) continue;
-    const int row = slot % p.c.page_size;
-    const T* k = static_cast<const T*>(p.c.k) + page * p.c.kp + hk * p.c.kh + row * p.c.kr;
-    const T* v = static_cast<const T*>(p.c.v) + page * p.c.vp + hk * p.c.vh + row * p.c.vr;
-    float s = 0.f;
-    for (int d = lane; d < D; d += 32) s = fmaf(to_f32(q[d]), to_f32(k[d]), s);
-    for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(~0u, s, x);
-    s *= p.scale_log2;
-    const float mn = fmaxf(m, s), f = m == mn ? 1.f : exp2f(m - mn), e = mn == -INFINITY ? 0.f : exp2f(s - mn);
-    m = mn;
-    l = l * f + e;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (lane + 32 * i < D) acc[i] = acc[i] * f + e * to_f32(v[lane + 32 * i]);
+// m[ROWS], l[ROWS], o[ROWS][D]
+template <int D, int ROWS> struct Partial {
+  static constexpr int kFloats = ROWS * (D + 2);
+  static __device__ __forceinline__ float* m(float* p) { return p; }
+  static __device__ __forceinline__ float* l(float* p) { return p + ROWS; }
+  static __device__ __forceinline__ float* o(float* p) { return p + 2 * ROWS; }
+};
+
+// The units of a sequence: those of its sinks that lie before the window's first, then the window's.
+struct Sequence {
+  int n, first, sinks, c0, a, units;
+  bool bad;
+};
+__device__ __forceinline__ Sequence sequence(const DecodeParams& p, int b) {
+  Sequence s;
+  s.bad = false;
+  s.n = paged_len(p.c, b, &s.bad);
+  const VisibleSlots v = visible_slots(s.n, p.W, p.S);
+  s.first = v.first;
+  s.sinks = v.sinks;
+  s.c0 = v.first / kUnit;
+  const int sink_units = (v.sinks + kUnit - 1) / kUnit;
+  s.a = sink_units < s.c0 ? sink_units : s.c0;
+  const int u = s.a + (s.n + kUnit - 1) / kUnit - s.c0;
+  s.units = u > 0 ? u : 1;  // an empty sequence has one, all masked, that writes its output
+  return s;
+}
+__device__ __forceinline__ int unit_chunk(const Sequence& s, int u) { return u < s.a ? u : u - s.a + s.c0; }
+
+// All units of all sequences, per (KV head, tile); every lane gets the sum.
+__device__ __forceinline__ int64_t lane_units(const DecodeParams& p, int lane, int* per_lane) {
+  const int per = (p.c.batch + 31) / 32;
+  *per_lane = per;
+  int64_t u = 0;
+  for (int i = 0; i < per; ++i) {
+    const int b = lane * per + i;
+    if (b < p.c.batch) u += sequence(p, b).units;
   }
-  __shared__ float sm[4], sl[4], sa[4][128];
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
+  return u;
+}
+__device__ __forceinline__ int64_t warp_sum(int64_t x) {
+  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
+  return x;
+}
+__device__ __forceinline__ int64_t warp_prefix(int64_t x, int lane) {  // exclusive
+  int64_t y = x;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t z = __shfl_up_sync(~0u, y, o);
+    if (lane >= o) y += z;
   }
-  for (int i = 0; i < 4; ++i) sa[warp][lane + 32 * i] = acc[i];
-  bad = __syncthreads_or(bad);
-  const float sink = p.sinks ? p.sinks[h] * kLog2e : -INFINITY;
-  float mm = sink;
-  for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm[w]);
-  const float base = mm == -INFINITY ? 0.f : mm;
-  float ll = exp2f(sink - base), oo = 0.f;
-  const int d = threadIdx.x;
-  for (int w = 0; w < 4; ++w) {
-    const float f = exp2f(sm[w] - base);
-    ll += sl[w] * f;
-    oo += sa[w][d] * f;
-  }
-  if (bad) {
-    ll = NAN;
-    if (d == 0) *p.c.page_error = 1;
-  }
-  if (d < D) static_cast<T*>(p.o)[b * p.ob + h * p.oh + d] = from_f32<T>(ll == 0.f ? 0.f : oo / ll);
-  if (d == 0) p.lse[(int64_t)b * p.Hq + h] = ll == 0.f ? -INFINITY : mm + log2f(ll);
+  return y - x;
 }
 
-// weights_out = decay * weights + the group's softmax weights, from the finished lse.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) weights_kernel(DecodeParams p) {
-  const int hk = blockIdx.y, b = blockIdx.z, G = p.Hq / p.c.n_kv_heads;
-  bool bad = false;
-  const int n = paged_len(p.c, b, &bad);
-  const VisibleSlots vis = visible_slots(n, p.W, p.S);
-  const int slot = blockIdx.x * kThreads + threadIdx.x;
-  if (slot >= n) return;
-  float w = p.c.weights ? p.decay * p.c.weights[b * p.c.wb + hk * p.c.wh + slot] : 0.f;
-  if (slot < vis.sinks || slot >= vis.first) {
-    const int page = paged_page(p.c, b, slot / p.c.page_size, &bad);
-    if (page >= 0) {
-      const T* k = static_cast<const T*>(p.c.k) + page * p.c.kp + hk * p.c.kh + slot % p.c.page_size * p.c.kr;
-      for (int g = 0; g < G; ++g) {
-        const int h = hk * G + g;
-        const T* q = static_cast<const T*>(p.q) + b * p.qb + h * p.qh;
-        float s = 0.f;
-        for (int d = 0; d < p.D; ++d) s = fmaf(to_f32(q[d]), to_f32(k[d]), s);
-        w += exp2f(s * p.scale_log2 - p.lse[(int64_t)b * p.Hq + h]);
+// Blocks that share `total` units: two units a warp at least, so that none of them is without any.
+__device__ __forceinline__ int active_blocks(int64_t total, int blocks) {
+  const int64_t n = (total + 2 * kWarps - 1) / (2 * kWarps);
+  return n < blocks ? (int)n : blocks;
+}
+
+// ---------------------------------------------------------------------------------------
+// tensor-core and copy primitives
+// ---------------------------------------------------------------------------------------
+template <typename T> __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma16816<__half>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+// 16 bytes to shared memory, zeros where !ok (then nothing is read)
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Byte offset of 16-byte piece `piece` of row `row` in a unit of 16 rows: pieces are swizzled so
+// that eight rows' equal pieces, an ldmatrix, lie in different banks.
+template <int D> __device__ __forceinline__ uint32_t swizzled(int row, int piece) {
+  constexpr int kPieces = D / 8;
+  const int x = D >= 64 ? (row & 7) : D == 32 ? ((row >> 1) & 3) : ((row >> 2) & 1);
+  return (uint32_t)(row * kPieces + (piece ^ x)) * 16;
+}
+
+// ---------------------------------------------------------------------------------------
+// A warp's walk over units [u0, u1) of one (sequence, KV head, tile)
+// ---------------------------------------------------------------------------------------
+template <typename T, int D, int ROWS> struct Walk {
+  static constexpr int kHalves = ROWS == 16 ? 2 : 1;  // rows of a thread: lane / 4 (+ 8)
+  static constexpr int kNt = D / 8, kKs = D / 16, kStages = Shape<D>::kStages;
+
+  float o[kNt][4];
+  float m[kHalves], l[kHalves];
+  bool bad;
+
+  __device__ __forceinline__ void run(const DecodeParams& p, uint32_t ring, int lane, int b, int hv, const Sequence& s,
+                                      int u0, int u1) {
+    const int h = hv / p.tiles, tile = hv % p.tiles;
+    const int g = lane / 4, t = lane % 4;
+    bad = s.bad;
+#pragma unroll
+    for (int i = 0; i < kNt; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kHalves; ++i) m[i] = -INFINITY, l[i] = 0.f;
+
+    const T* kbase = static_cast<const T*>(p.c.k) + h * p.c.kh;
+    const T* vbase = static_cast<const T*>(p.c.v) + h * p.c.vh;
+
+    // page of unit u0 + 32 i + lane, looked up 32 units at a time
+    auto pages = [&](int u) -> int {
+      if (u >= u1) return -1;
+      const int chunk = unit_chunk(s, u);
+      if (chunk * kUnit >= s.n) return -1;
+      return paged_page(p.c, b, chunk / p.units_per_page, &bad);
+    };
+    int ids = pages(u0 + lane);
+    const int upp = p.units_per_page;
+
+    auto issue = [&](int u) {
+      if (u < u1) {
+        const int i = u - u0;
+        if (i && (i & 31) == 0) ids = pages(u + lane);
+        const int page = __shfl_sync(~0u, ids, i & 31);
+        const int chunk = unit_chunk(s, u), slot0 = chunk * kUnit, row0 = (chunk % upp) * kUnit;
+        const T* kp = kbase + (page < 0 ? 0 : page) * p.c.kp + (int64_t)row0 * p.c.kr;
+        const T* vp = vbase + (page < 0 ? 0 : page) * p.c.vp + (int64_t)row0 * p.c.vr;
+        const uint32_t dst = ring + (uint32_t)(i % kStages) * Shape<D>::kUnitBytes;
+        constexpr int kPieces = D / 8;
+#pragma unroll
+        for (int e = 0; e < kUnit * kPieces; e += 32) {
+          const int at = e + lane, row = at / kPieces, piece = at % kPieces, slot = slot0 + row;
+          const bool ok = page >= 0 && slot < s.n && (slot >= s.first || slot < s.sinks);
+          copy16(dst + swizzled<D>(row, piece), kp + row * p.c.kr + piece * 8, ok);
+          copy16(dst + kUnit * D * 2 + swizzled<D>(row, piece), vp + row * p.c.vr + piece * 8, ok);
+        }
       }
+      copy_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) issue(u0 + i);
+
+    // Q as the A operand, rows past the group's heads as zeros
+    uint32_t qa[kKs][4];
+#pragma unroll
+    for (int ks = 0; ks < kKs; ++ks)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = g + (r & 1) * 8, col = ks * 16 + (r >> 1) * 8 + 2 * t;
+        const int head = tile * ROWS + row;
+        qa[ks][r] = row < ROWS && head < p.G
+                        ? *reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.q) + b * p.qb +
+                                                             (int64_t)(h * p.G + head) * p.qh + col)
+                        : 0u;
+      }
+
+    for (int u = u0; u < u1; ++u) {
+      issue(u + kStages - 1);
+      copy_wait<kStages - 1>();
+      __syncwarp();
+      const uint32_t kt = ring + (uint32_t)((u - u0) % kStages) * Shape<D>::kUnitBytes, vt = kt + kUnit * D * 2;
+      float sc[2][4] = {};
+#pragma unroll
+      for (int ks = 0; ks < kKs; ++ks) {
+        uint32_t kb[4];
+        ldsm4(kb, kt + swizzled<D>((lane >> 4) * 8 + (lane & 7), ks * 2 + ((lane >> 3) & 1)));
+        mma16816<T>(sc[0], qa[ks], kb[0], kb[1]);
+        mma16816<T>(sc[1], qa[ks], kb[2], kb[3]);
+      }
+      const int slot0 = unit_chunk(s, u) * kUnit;
+      const bool full = slot0 + kUnit <= s.n && (slot0 >= s.first || slot0 + kUnit <= s.sinks);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int slot = slot0 + 8 * j + 2 * t + e;
+          const bool ok = full || (slot < s.n && (slot >= s.first || slot < s.sinks));
+#pragma unroll
+          for (int r = 0; r < kHalves; ++r) sc[j][2 * r + e] = ok ? sc[j][2 * r + e] * p.scale_log2 : -INFINITY;
+        }
+      if (p.scores) {
+        float* out = p.scores + (((int64_t)b * p.c.n_kv_heads * p.tiles + hv) * p.max_units + u) * (ROWS * kUnit);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int r = 0; r < kHalves; ++r)
+            *reinterpret_cast<float2*>(out + (g + 8 * r) * kUnit + 8 * j + 2 * t) =
+                make_float2(sc[j][2 * r], sc[j][2 * r + 1]);
+      }
+      float up[kHalves];
+      bool grew = false;
+#pragma unroll
+      for (int r = 0; r < kHalves; ++r) {
+        float x = fmaxf(max3f(sc[0][2 * r], sc[0][2 * r + 1], sc[1][2 * r]), sc[1][2 * r + 1]);
+        x = fmaxf(x, __shfl_xor_sync(~0u, x, 1));
+        x = fmaxf(x, __shfl_xor_sync(~0u, x, 2));
+        up[r] = fmaxf(m[r], x);
+        grew |= up[r] > m[r];
+      }
+      if (__any_sync(~0u, grew)) {
+#pragma unroll
+        for (int r = 0; r < kHalves; ++r) {
+          const float f = up[r] > m[r] ? fast_exp2(m[r] - up[r]) : 1.f;
+          m[r] = up[r];
+          l[r] *= f;
+          if (kHalves == 1) {  // both halves of the tile are this row: its hi and its lo sums
+#pragma unroll
+            for (int i = 0; i < kNt; ++i) o[i][0] *= f, o[i][1] *= f, o[i][2] *= f, o[i][3] *= f;
+          } else {
+#pragma unroll
+            for (int i = 0; i < kNt; ++i) o[i][2 * r] *= f, o[i][2 * r + 1] *= f;
+          }
+        }
+      }
+      uint32_t hi[kHalves][2], lo[kHalves][2];
+#pragma unroll
+      for (int r = 0; r < kHalves; ++r) {
+        const float base = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float x = fast_exp2(sc[j][2 * r] - base), y = fast_exp2(sc[j][2 * r + 1] - base);
+          l[r] += x + y;
+          hi[r][j] = Pack<T>::pack(x, y);
+          const T* q = reinterpret_cast<const T*>(&hi[r][j]);
+          lo[r][j] = Pack<T>::pack(x - Pack<T>::to(q[0]), y - Pack<T>::to(q[1]));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kNt; i += 2) {
+        uint32_t vb[4];
+        ldsm4t(vb, vt + swizzled<D>(((lane >> 3) & 1) * 8 + (lane & 7), i + (lane >> 4)));
+        if (kHalves == 1) {
+          const uint32_t a[4] = {hi[0][0], lo[0][0], hi[0][1], lo[0][1]};
+          mma16816<T>(o[i], a, vb[0], vb[1]);
+          mma16816<T>(o[i + 1], a, vb[2], vb[3]);
+        } else {
+          const uint32_t a[4] = {hi[0][0], hi[kHalves - 1][0], hi[0][1], hi[kHalves - 1][1]};
+          const uint32_t c[4] = {lo[0][0], lo[kHalves - 1][0], lo[0][1], lo[kHalves - 1][1]};
+          mma16816<T>(o[i], a, vb[0], vb[1]);
+          mma16816<T>(o[i + 1], a, vb[2], vb[3]);
+          mma16816<T>(o[i], c, vb[0], vb[1]);
+          mma16816<T>(o[i + 1], c, vb[2], vb[3]);
+        }
+      }
+      __syncwarp();
+    }
+    copy_wait<0>();
+    __syncwarp();
+    bad = __any_sync(~0u, bad);
+#pragma unroll
+    for (int r = 0; r < kHalves; ++r) {
+      l[r] += __shfl_xor_sync(~0u, l[r], 1);
+      l[r] += __shfl_xor_sync(~0u, l[r], 2);
+      if (bad) l[r] = NAN;
+    }
+    if (kHalves == 1)
+#pragma unroll
+      for (int i = 0; i < kNt; ++i) o[i][0] += o[i][2], o[i][1] += o[i][3];
+    if (bad && lane == 0) *p.c.page_error = 1;
+  }
+
+  __device__ __forceinline__ void store(float* part, int lane) const {
+    using P = Partial<D, ROWS>;
+    const int g = lane / 4, t = lane % 4;
+#pragma unroll
+    for (int r = 0; r < kHalves; ++r) {
+      if (t == 0) {
+        P::m(part)[g + 8 * r] = m[r];
+        P::l(part)[g + 8 * r] = l[r];
+      }
+#pragma unroll
+      for (int i = 0; i < kNt; ++i)
+        *reinterpret_cast<float2*>(P::o(part) + (g + 8 * r) * D + 8 * i + 2 * t) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
     }
   }
+};
+
+// A finished row's output and log-sum-exp from its joined maximum, sum and value.
+struct Row {
+  float inv, lse;
+};
+__device__ __forceinline__ Row finish(float m, float l, float sink) {
+  const float top = fmaxf(m, sink), base = top == -INFINITY ? 0.f : top;
+  const float f = fast_exp2(m - base), total = l * f + fast_exp2(sink - base);
+  Row r;
+  r.inv = total == 0.f ? 0.f : f / total;
+  r.lse = total == 0.f ? -INFINITY : top + log2f(total);
+  return r;
+}
+
+// Joins `count` partials at part(0 ..) of one (sequence, KV head, tile): into the output, or into
+// `into` where it is given.  All threads of the block, D values of a row by neighbouring threads.
+template <typename T, int D, int ROWS, int THREADS, typename F>
+__device__ __forceinline__ void join(const DecodeParams& p, int b, int hv, int count, F part, float* into) {
+  using P = Partial<D, ROWS>;
+  const int h = hv / p.tiles, tile = hv % p.tiles;
+  const int rows = p.G - tile * ROWS < ROWS ? p.G - tile * ROWS : ROWS;
+  for (int e = threadIdx.x; e < rows * (D / 2); e += THREADS) {
+    const int r = e / (D / 2), d = e % (D / 2) * 2;
+    float m = -INFINITY;
+    for (int i = 0; i < count; ++i) m = fmaxf(m, P::m(part(i))[r]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f, x = 0.f, y = 0.f;
+    for (int i = 0; i < count; ++i) {
+      float* q = part(i);
+      const float f = fast_exp2(P::m(q)[r] - base);
+      const float2 v = *reinterpret_cast<const float2*>(P::o(q) + r * D + d);
+      l = fmaf(P::l(q)[r], f, l);
+      x = fmaf(v.x, f, x);
+      y = fmaf(v.y, f, y);
+    }
+    if (into) {
+      if (d == 0) {
+        P::m(into)[r] = m;
+        P::l(into)[r] = l;
+      }
+      *reinterpret_cast<float2*>(P::o(into) + r * D + d) = make_float2(x, y);
+    } else {
+      const int head = h * p.G + tile * ROWS + r;
+      const Row w = finish(m, l, p.sinks ? p.sinks[head] * kLog2e : -INFINITY);
+      *reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.ob + head * p.oh + d) = Pack<T>::pack(x * w.inv, y * w.inv);
+      if (p.lse && d == 0) p.lse[(int64_t)b * p.Hq + head] = w.lse;
+    }
+  }
+}
+
+struct Piece {
+  int bh, u0, u1, units;
+};
+
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kernel(DecodeParams p) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ Piece pieces[kWarps][2];
+  using P = Partial<D, ROWS>;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int vh = p.c.n_kv_heads * p.tiles;
+  unsigned char* ring = smem + warp * Shape<D>::kRing;
+  float* last = reinterpret_cast<float*>(ring);
+  float* first = p.whole ? nullptr : p.heads + ((int64_t)blockIdx.x * kWarps + warp) * P::kFloats;
+  sm100::pdl_trigger();
+  if (lane < 2) pieces[warp][lane].bh = -1;
+  __syncwarp();
+
+  // this warp's range: units [u, ...) of (b, hv), `todo` of them
+  int b, hv, u;
+  int64_t todo;
+  Sequence s;
+  if (p.whole) {
+    b = blockIdx.x / vh;
+    hv = blockIdx.x % vh;
+    s = sequence(p, b);
+    u = (int)((int64_t)s.units * warp / kWarps);
+    todo = (int64_t)s.units * (warp + 1) / kWarps - u;
+  } else {
+    int per;
+    const int64_t mine = lane_units(p, lane, &per);
+    const int64_t total = warp_sum(mine) * vh, before = warp_prefix(mine, lane) * vh;
+    const int blocks = active_blocks(total, gridDim.x);
+    if ((int)blockIdx.x >= blocks) return;
+    const int64_t b0 = total * blockIdx.x / blocks, b1 = total * (blockIdx.x + 1) / blocks;
+    const int64_t start = b0 + (b1 - b0) * warp / kWarps;
+    todo = b0 + (b1 - b0) * (warp + 1) / kWarps - start;
+    // the lane whose sequences hold `start`, then the sequence
+    const unsigned has = __ballot_sync(~0u, start >= before && start < before + mine * vh);
+    const int src = has ? __ffs(has) - 1 : 0;
+    int64_t rest = start - __shfl_sync(~0u, before, src);
+    b = src * per;
+    s = sequence(p, b);
+    while (todo > 0 && rest >= (int64_t)s.units * vh) {
+      rest -= (int64_t)s.units * vh;
+      s = sequence(p, ++b);
+    }
+    hv = (int)(rest / s.units);
+    u = (int)(rest % s.units);
+  }
+  Walk<T, D, ROWS> w;
+  while (todo > 0) {
+    const int u1 = (int)(todo < s.units - u ? u + todo : s.units);
+    w.run(p, saddr(ring), lane, b, hv, s, u, u1);
+    todo -= u1 - u;
+    // a piece of its own that something follows goes out through `first`, the last one stays here
+    const bool more = todo > 0;
+    if (more && u == 0) {  // whole, and done: finish it
+      w.store(last, lane);
+      __syncwarp();
+      // (one warp joins its only partial)
+      const int h = hv / p.tiles, tile = hv % p.tiles;
+      const int rows = p.G - tile * ROWS < ROWS ? p.G - tile * ROWS : ROWS;
+      for (int e = lane; e < rows * (D / 2); e += 32) {
+        const int r = e / (D / 2), d = e % (D / 2) * 2, head = h * p.G + tile * ROWS + r;
+        const Row f = finish(P::m(last)[r], P::l(last)[r], p.sinks ? p.sinks[head] * kLog2e : -INFINITY);
+        const float2 v = *reinterpret_cast<const float2*>(P::o(last) + r * D + d);
+        *reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.ob + head * p.oh + d) =
+            Pack<T>::pack(v.x * f.inv, v.y * f.inv);
+        if (p.lse && d == 0) p.lse[(int64_t)b * p.Hq + head] = f.lse;
+      }
+      __syncwarp();
+    } else {
+      w.store(more ? first : last, lane);
+      if (lane == 0) pieces[warp][more ? 0 : 1] = {b * vh + hv, u, u1, s.units};
+    }
+    u = 0;
+    if (more && ++hv == vh) {
+      hv = 0;
+      s = sequence(p, ++b);
+    }
+  }
+  __syncthreads();
+
+  // join neighbouring pieces of the same (sequence, KV head, tile)
+  for (int i = 0; i < 2 * kWarps;) {
+    const Piece a = pieces[i / 2][i % 2];
+    if (a.bh < 0) {
+      ++i;
+      continue;
+    }
+    int at[2 * kWarps], count = 0, end = a.u1;
+    at[count++] = i++;
+    for (; i < 2 * kWarps; ++i) {
+      const Piece& c = pieces[i / 2][i % 2];
+      if (c.bh < 0) continue;
+      if (c.bh != a.bh) break;
+      at[count++] = i;
+      end = c.u1;
+    }
+    const bool done = a.u0 == 0 && end == a.units;
+    float* into = done ? nullptr : p.partials + ((int64_t)blockIdx.x * 2 + (a.u0 > 0 ? 0 : 1)) * P::kFloats;
+    auto part = [&](int k) -> float* {
+      const int x = at[k];
+      return x % 2 ? reinterpret_cast<float*>(smem + x / 2 * Shape<D>::kRing)
+                   : p.heads + ((int64_t)blockIdx.x * kWarps + x / 2) * P::kFloats;
+    };
+    join<T, D, ROWS, kThreads>(p, a.bh / vh, a.bh % vh, count, part, into);
+  }
+}
+
+// The sequences that span blocks: a block per (sequence, KV head, tile) finds the blocks that hold
+// it by the same dealing out, and joins their partials.
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(DecodeParams p, int grid) {
+  using P = Partial<D, ROWS>;
+  const int lane = threadIdx.x % 32, vh = p.c.n_kv_heads * p.tiles;
+  const int b = blockIdx.x / vh, hv = blockIdx.x % vh;
+  int64_t all = 0, before = 0;
+  for (int i = lane; i < p.c.batch; i += 32) {
+    const int n = sequence(p, i).units;
+    all += n;
+    if (i < b) before += n;
+  }
+  const int64_t total = warp_sum(all) * vh;
+  const int units = sequence(p, b).units, blocks = active_blocks(total, grid);
+  const int64_t start = warp_sum(before) * vh + (int64_t)hv * units, end = start + units;
+  // block c holds [total c / blocks, total (c + 1) / blocks)
+  const int c0 = (int)(((start + 1) * blocks - 1) / total), c1 = (int)((end * blocks - 1) / total);
+  sm100::pdl_wait();
+  if (c0 == c1) return;
+  auto part = [&](int i) -> float* {
+    const int c = c0 + i;
+    const int64_t from = total * c / blocks;
+    return p.partials + ((int64_t)c * 2 + (from > start ? 0 : 1)) * P::kFloats;
+  };
+  join<T, D, ROWS, kJoinThreads>(p, b, hv, c1 - c0 + 1, part, nullptr);
+}
+
+// weights_out = decay * weights + the group's softmax weights, exp2 of the stored scores less the
+// finished log-sum-exp.
+template <int ROWS>
+__global__ void __launch_bounds__(kWeightThreads) weights_kernel(DecodeParams p, int tiles_x) {
+  const int hk = blockIdx.x / tiles_x % p.c.n_kv_heads, b = blockIdx.x / tiles_x / p.c.n_kv_heads;
+  const Sequence s = sequence(p, b);
+  const int slot = blockIdx.x % tiles_x * kWeightThreads + threadIdx.x;
+  if (slot >= s.n) return;
+  float w = p.c.weights ? p.decay * p.c.weights[b * p.c.wb + hk * p.c.wh + slot] : 0.f;
+  sm100::pdl_wait();
+  if (slot < s.sinks || slot >= s.first) {
+    const int chunk = slot / kUnit, u = chunk < s.a ? chunk : chunk - s.c0 + s.a;
+    float sum = 0.f;
+    for (int tile = 0; tile < p.tiles; ++tile) {
+      const int rows = p.G - tile * ROWS < ROWS ? p.G - tile * ROWS : ROWS;
+      const float* sc = p.scores + ((((int64_t)b * p.c.n_kv_heads + hk) * p.tiles + tile) * p.max_units + u) * (ROWS * kUnit) +
+                        slot % kUnit;
+      const float* lse = p.lse + (int64_t)b * p.Hq + hk * p.G + tile * ROWS;
+      for (int r = 0; r < rows; ++r) sum += fast_exp2(sc[r * kUnit] - lse[r]);
+    }
+    w += sum;
+  }
   p.wout[b * p.wob + hk * p.woh + slot] = w;
+}
+
+// What a call needs of the workspace, in floats each, every part a multiple of 64.
+struct Plan {
+  int rows, tiles, max_units, whole, blocks;
+  size_t lse, partials, heads, scores;
+};
+size_t round64(size_t n) { return (n + 63) & ~(size_t)63; }
+
+// Visible units from which a sequence is split: below, a block of its own is as quick as a split
+// and saves the join.
+constexpr int kWholeUnits = 32;
+
+Plan plan(const SwaPagedDecodeArgs& a) {
+  const SwaPagedKV& c = a.cache;
+  const int G = a.n_q_heads / c.n_kv_heads, D = c.head_dim;
+  Plan r = {};
+  r.rows = G <= 8 ? 8 : 16;
+  r.tiles = (G + r.rows - 1) / r.rows;
+  const int64_t cap = (int64_t)c.max_pages * c.page_size;
+  int64_t units = (cap + kUnit - 1) / kUnit;
+  const int64_t w = a.window_size > 0 ? a.window_size : 0;
+  // the sinks' units, the window's, and one more where it begins inside a unit
+  const int64_t bound = ((int64_t)a.sink_size + kUnit - 1) / kUnit + (w + kUnit - 1) / kUnit + 1;
+  if (bound < units) units = bound;
+  r.max_units = units > 0 ? (int)units : 1;
+  const int64_t vh = (int64_t)c.n_kv_heads * r.tiles, seqs = vh * c.batch;
+  r.whole = r.max_units <= kWholeUnits;
+  const int most = D == 128 ? Shape<128>::kMaxBlocks : Shape<64>::kMaxBlocks;
+  // at least two units a warp
+  const int64_t want = (seqs * r.max_units + 2 * kWarps - 1) / (2 * kWarps);
+  r.blocks = (int)(r.whole ? seqs : want < most ? want : most);
+  const size_t part = (size_t)r.rows * (D + 2);
+  r.lse = a.weights_out && !a.lse ? round64((size_t)c.batch * a.n_q_heads) : 0;
+  r.partials = r.whole ? 0 : round64(2 * part * r.blocks);
+  r.heads = r.whole ? 0 : round64(kWarps * part * r.blocks);
+  r.scores = a.weights_out ? round64((size_t)seqs * r.max_units * r.rows * kUnit) : 0;
+  return r;
+}
+
+template <typename T, int D, int ROWS>
+cudaError_t launch(const DecodeParams& p, const Plan& pl, cudaStream_t st) {
+  constexpr int smem = kWarps * Shape<D>::kRing;
+  auto kern = decode_kernel<T, D, ROWS>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  kern<<<pl.blocks, kThreads, smem, st>>>(p);
+  e = cudaGetLastError();
+  const int seqs = p.c.batch * p.c.n_kv_heads * p.tiles;
+  if (e == cudaSuccess && !p.whole)
+    e = launch_pdl(join_kernel<T, D, ROWS>, seqs, kJoinThreads, 0, st, p, pl.blocks);
+  if (e == cudaSuccess && p.wout) {
+    const int x = (p.c.max_pages * p.c.page_size + kWeightThreads - 1) / kWeightThreads;
+    if (x > 0) e = launch_pdl(weights_kernel<ROWS>, x * p.c.n_kv_heads * p.c.batch, kWeightThreads, 0, st, p, x);
+  }
+  return e;
+}
+
+template <typename T, int ROWS>
+cudaError_t launch_dim(int D, const DecodeParams& p, const Plan& pl, cudaStream_t st) {
+  switch (D) {
+    case 16: return launch<T, 16, ROWS>(p, pl, st);
+    case 32: return launch<T, 32, ROWS>(p, pl, st);
+    case 64: return launch<T, 64, ROWS>(p, pl, st);
+    default: return launch<T, 128, ROWS>(p, pl, st);
+  }
 }
 
 }  // namespace
 
 size_t paged_decode_workspace(const SwaPagedDecodeArgs& a) {
-  return ((size_t)a.cache.batch * a.n_q_heads * sizeof(float) + 255) & ~(size_t)255;
-}
-
-template <typename T>
-static cudaError_t launch(const DecodeParams& p, cudaStream_t st) {
-  decode_kernel<T><<<dim3(p.Hq, p.c.batch), kThreads, 0, st>>>(p);
-  if (p.wout) {
-    const int cap = p.c.max_pages * p.c.page_size;
-    weights_kernel<T><<<dim3((cap + kThreads - 1) / kThreads, p.c.n_kv_heads, p.c.batch), kThreads, 0, st>>>(p);
-  }
-  return cudaGetLastError();
+  const Plan r = plan(a);
+  return (r.lse + r.partials + r.heads + r.scores) * sizeof(float);
 }
 
 cudaError_t launch_paged_decode(const PagedParams& c, const SwaPagedDecodeArgs& a, cudaStream_t st) {
+  const Plan pl = plan(a);
   DecodeParams p;
   p.c = c;
-  p.Hq = a.n_q_heads; p.W = a.window_size; p.S = a.sink_size; p.D = a.cache.head_dim;
+  p.Hq = a.n_q_heads; p.G = a.n_q_heads / c.n_kv_heads; p.tiles = pl.tiles;
+  p.W = a.window_size; p.S = a.sink_size;
+  p.units_per_page = c.page_size / kUnit;
+  p.max_units = pl.max_units; p.whole = pl.whole;
   p.scale_log2 = a.softmax_scale * kLog2e;
   p.q = a.q.ptr; p.o = a.o.ptr;
   p.qb = a.q.stride_t; p.qh = a.q.stride_h; p.ob = a.o.stride_t; p.oh = a.o.stride_h;
-  p.lse = a.lse ? a.lse : static_cast<float*>(a.workspace);
+  float* ws = static_cast<float*>(a.workspace);
+  p.lse = a.lse ? a.lse : pl.lse ? ws : nullptr;
+  p.partials = ws + pl.lse;
+  p.heads = p.partials + pl.partials;
+  p.scores = pl.scores ? p.heads + pl.heads : nullptr;
   p.sinks = a.sink_logits;
   p.wout = a.weights_out; p.wob = a.wo_stride_b; p.woh = a.wo_stride_h;
   p.decay = a.decay;
-  return a.cache.dtype == SWA_F16 ? launch<__half>(p, st) : launch<__nv_bfloat16>(p, st);
+  if (a.cache.dtype == SWA_F16)
+    return pl.rows == 8 ? launch_dim<__half, 8>(a.cache.head_dim, p, pl, st) : launch_dim<__half, 16>(a.cache.head_dim, p, pl, st);
+  return pl.rows == 8 ? launch_dim<__nv_bfloat16, 8>(a.cache.head_dim, p, pl, st)
+                      : launch_dim<__nv_bfloat16, 16>(a.cache.head_dim, p, pl, st);
 }
 
 }  // namespace swa

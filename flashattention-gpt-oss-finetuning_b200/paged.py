@@ -194,15 +194,16 @@ class PagedKVCache:
             _lib.check(_lib.lib().swa_paged_append(ctypes.byref(args), _stream(self._dev)), "swa_paged_append")
         return out
 
-    def _decode_plan(self, hq: int, weigh: bool):
-        """Argument block and workspace size for this number of query heads."""
-        plan = self._plans.get((hq, weigh))
+    def _decode_plan(self, hq: int, window: int, sinks: int, weigh: bool):
+        """Argument block and workspace size for this number of query heads and this mask."""
+        key = (hq, window, sinks, weigh)
+        plan = self._plans.get(key)
         if plan is None:
             if hq <= 0 or hq % self._hkv:
                 raise ValueError("Number of query heads must be divisible by number of K/V heads")
-            args = _lib.SwaPagedDecodeArgs(self._c, hq)
-            args.weights_out = 256 if weigh else None
-            plan = self._plans[hq, weigh] = (args, _lib.lib().swa_paged_decode_workspace_size(ctypes.byref(args)))
+            args = _lib.SwaPagedDecodeArgs(self._c, hq, window, sinks)
+            args.weights_out = 256 if weigh else None  # its size counts, its address not yet
+            plan = self._plans[key] = (args, _lib.lib().swa_paged_decode_workspace_size(ctypes.byref(args)))
         return plan
 
     def decode(self, q: torch.Tensor, window_size: Optional[int] = None, sink_size: int = 0,
@@ -220,13 +221,12 @@ class PagedKVCache:
         if q.shape[0] != self._b:
             raise ValueError(f"q must hold one token for each of {self._b} sequences; got {q.shape[0]}")
         hq, dev = q.shape[1], self._dev
-        plan, ws_bytes = self._decode_plan(hq, weights_out is not None)
+        window = _WHOLE if window_size is None else max(-1, min(int(window_size), _WHOLE))
+        plan, ws_bytes = self._decode_plan(hq, window, min(int(sink_size), _WHOLE), weights_out is not None)
         if not _rows_ok(q):
             q = q.clone(memory_format=torch.contiguous_format)
         o = torch.empty((self._b, hq, self._d), device=dev, dtype=self._dtype)
         args = _lib.SwaPagedDecodeArgs.from_buffer_copy(plan)
-        args.window_size = _WHOLE if window_size is None else max(-1, min(int(window_size), _WHOLE))
-        args.sink_size = min(int(sink_size), _WHOLE)
         args.softmax_scale = 1.0 / math.sqrt(self._d) if softmax_scale is None else float(softmax_scale)
         args.q, args.o = _packed(q), _packed(o)
         lse = torch.empty((self._b, hq), device=dev, dtype=torch.float32) if return_lse else None

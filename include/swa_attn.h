@@ -304,8 +304,8 @@ typedef struct SwaPagedDecodeArgs {
  * head h of their softmax weight on slot j (0 where it is not visible), for j < n. */
 SWA_API int swa_paged_decode(const SwaPagedDecodeArgs* args, void* stream);
 
-/* Scratch that swa_paged_decode needs (pointers are not looked at, except weights_out for
- * NULL). */
+/* Scratch that swa_paged_decode needs, by the sizes, the window and the sinks (of the pointers
+ * it matters whether lse and weights_out are NULL); may be 0. */
 SWA_API size_t swa_paged_decode_workspace_size(const SwaPagedDecodeArgs* args);
 
 typedef struct SwaPagedEvictArgs {
