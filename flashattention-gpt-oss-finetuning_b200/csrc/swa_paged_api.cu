@@ -132,7 +132,7 @@ int swa_paged_decode(const SwaPagedDecodeArgs* a, void* stream) {
   swa::PagedParams c;
   if (int st = build_cache(a->cache, &c)) return st;
   if (a->n_q_heads <= 0 || a->n_q_heads % c.n_kv_heads || a->sink_size < 0) return SWA_ERR_INVALID_ARG;
-  if ((int64_t)c.batch * a->n_q_heads > INT32_MAX / 1024) return SWA_ERR_UNSUPPORTED;
+  if ((int64_t)c.batch * (a->n_q_heads + 16 * (int64_t)c.n_kv_heads) > INT32_MAX / 64) return SWA_ERR_UNSUPPORTED;
   if (!(a->softmax_scale == a->softmax_scale) || !(a->decay == a->decay)) return SWA_ERR_INVALID_ARG;
   if (c.batch == 0) return SWA_OK;
   if (!packed_ok(a->q) || !packed_ok(a->o)) return SWA_ERR_INVALID_ARG;
@@ -140,8 +140,8 @@ int swa_paged_decode(const SwaPagedDecodeArgs* a, void* stream) {
   if (!aligned16(a->o.ptr) || a->o.stride_t % 8 || a->o.stride_h % 8) return SWA_ERR_UNSUPPORTED;
   if (a->weights_out) {
     if (a->wo_stride_b < 0 || a->wo_stride_h < 0) return SWA_ERR_UNSUPPORTED;
-    // a thread per slot and KV head, 256 to a block
-    if (((int64_t)c.max_pages * c.page_size / 256 + 1) * c.n_kv_heads * c.batch > INT32_MAX) return SWA_ERR_UNSUPPORTED;
+    // a block per 512 slots of a KV head, in one grid
+    if (((int64_t)c.max_pages * c.page_size / 512 + 1) * c.n_kv_heads * c.batch > INT32_MAX / 2) return SWA_ERR_UNSUPPORTED;
   }
   if (int st = check_workspace(a->workspace, a->workspace_bytes, swa_paged_decode_workspace_size(a))) return st;
   if (int st = bind_flag(&c)) return st;

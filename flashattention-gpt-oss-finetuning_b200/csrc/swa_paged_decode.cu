@@ -33,8 +33,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kUnit = 16;     // slots per unit
 constexpr int kSms = 148;
-constexpr int kJoinThreads = 128;
-constexpr int kWeightThreads = 256;
+constexpr int kWeightSlots = 512;  // slots per block of finish_kernel
 
 template <int D> struct Shape {
   static constexpr int kUnitBytes = 2 * kUnit * D * 2;  // K and V
@@ -49,7 +48,7 @@ struct DecodeParams {
   int Hq, G, tiles, W, S;  // tiles: row tiles per KV head
   int units_per_page;
   int max_units;           // bound on the units of a sequence
-  int whole;               // 1: a block per (sequence, KV head, tile)
+  int warps;               // warps per (sequence, KV head, tile), 1 or kWarps; 0: dealt out
   float scale_log2;
   const void* q; void* o;
   int64_t qb, qh, ob, oh;
@@ -60,7 +59,7 @@ struct DecodeParams {
   float decay;
   float* partials;         // [blocks][2] Partial
   float* heads;            // [blocks][warps] Partial: the first piece of a warp that has two
-  float* scores;           // [B * Hkv * tiles][max_units][ROWS][16]
+  float* scores;           // [B * Hkv * tiles][max_units][16][ROWS]
 };
 
 // m[ROWS], l[ROWS], o[ROWS][D]
@@ -164,6 +163,19 @@ template <int D> __device__ __forceinline__ uint32_t swizzled(int row, int piece
   return (uint32_t)(row * kPieces + (piece ^ x)) * 16;
 }
 
+// A finished row's output and log-sum-exp from its joined maximum, sum and value.
+struct Row {
+  float inv, lse;
+};
+__device__ __forceinline__ Row finish(float m, float l, float sink) {
+  const float top = fmaxf(m, sink), base = top == -INFINITY ? 0.f : top;
+  const float f = fast_exp2(m - base), total = l * f + fast_exp2(sink - base);
+  Row r;
+  r.inv = total == 0.f ? 0.f : f / total;
+  r.lse = total == 0.f ? -INFINITY : top + log2f(total);
+  return r;
+}
+
 // ---------------------------------------------------------------------------------------
 // A warp's walk over units [u0, u1) of one (sequence, KV head, tile)
 // ---------------------------------------------------------------------------------------
@@ -265,8 +277,8 @@ template <typename T, int D, int ROWS> struct Walk {
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int r = 0; r < kHalves; ++r)
-            *reinterpret_cast<float2*>(out + (g + 8 * r) * kUnit + 8 * j + 2 * t) =
-                make_float2(sc[j][2 * r], sc[j][2 * r + 1]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) out[(8 * j + 2 * t + e) * ROWS + g + 8 * r] = sc[j][2 * r + e];
       }
       float up[kHalves];
       bool grew = false;
@@ -354,29 +366,33 @@ template <typename T, int D, int ROWS> struct Walk {
         *reinterpret_cast<float2*>(P::o(part) + (g + 8 * r) * D + 8 * i + 2 * t) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
     }
   }
+
+  // The output of a (sequence, KV head, tile) that this warp has walked whole.
+  __device__ __forceinline__ void write(const DecodeParams& p, int lane, int b, int hv) const {
+    const int h = hv / p.tiles, tile = hv % p.tiles, g = lane / 4, t = lane % 4;
+#pragma unroll
+    for (int r = 0; r < kHalves; ++r) {
+      const int row = tile * ROWS + g + 8 * r, head = h * p.G + row;
+      if (row < p.G) {
+        const Row f = finish(m[r], l[r], p.sinks ? p.sinks[head] * kLog2e : -INFINITY);
+        T* out = static_cast<T*>(p.o) + b * p.ob + head * p.oh + 2 * t;
+#pragma unroll
+        for (int i = 0; i < kNt; ++i)
+          *reinterpret_cast<uint32_t*>(out + 8 * i) = Pack<T>::pack(o[i][2 * r] * f.inv, o[i][2 * r + 1] * f.inv);
+        if (p.lse && t == 0) p.lse[(int64_t)b * p.Hq + head] = f.lse;
+      }
+    }
+  }
 };
 
-// A finished row's output and log-sum-exp from its joined maximum, sum and value.
-struct Row {
-  float inv, lse;
-};
-__device__ __forceinline__ Row finish(float m, float l, float sink) {
-  const float top = fmaxf(m, sink), base = top == -INFINITY ? 0.f : top;
-  const float f = fast_exp2(m - base), total = l * f + fast_exp2(sink - base);
-  Row r;
-  r.inv = total == 0.f ? 0.f : f / total;
-  r.lse = total == 0.f ? -INFINITY : top + log2f(total);
-  return r;
-}
-
-// Joins `count` partials at part(0 ..) of one (sequence, KV head, tile): into the output, or into
-// `into` where it is given.  All threads of the block, D values of a row by neighbouring threads.
-template <typename T, int D, int ROWS, int THREADS, typename F>
+// Joins `count` partials at part(0 ..) of one (sequence, KV head, tile) by all threads of the block:
+// into the output, or into `into` where it is given.
+template <typename T, int D, int ROWS, typename F>
 __device__ __forceinline__ void join(const DecodeParams& p, int b, int hv, int count, F part, float* into) {
   using P = Partial<D, ROWS>;
   const int h = hv / p.tiles, tile = hv % p.tiles;
   const int rows = p.G - tile * ROWS < ROWS ? p.G - tile * ROWS : ROWS;
-  for (int e = threadIdx.x; e < rows * (D / 2); e += THREADS) {
+  for (int e = threadIdx.x; e < rows * (D / 2); e += kThreads) {
     const int r = e / (D / 2), d = e % (D / 2) * 2;
     float m = -INFINITY;
     for (int i = 0; i < count; ++i) m = fmaxf(m, P::m(part(i))[r]);
@@ -417,22 +433,21 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kerne
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int vh = p.c.n_kv_heads * p.tiles;
   unsigned char* ring = smem + warp * Shape<D>::kRing;
-  float* last = reinterpret_cast<float*>(ring);
-  float* first = p.whole ? nullptr : p.heads + ((int64_t)blockIdx.x * kWarps + warp) * P::kFloats;
   sm100::pdl_trigger();
-  if (lane < 2) pieces[warp][lane].bh = -1;
-  __syncwarp();
 
   // this warp's range: units [u, ...) of (b, hv), `todo` of them
   int b, hv, u;
   int64_t todo;
   Sequence s;
-  if (p.whole) {
-    b = blockIdx.x / vh;
-    hv = blockIdx.x % vh;
+  if (p.warps) {
+    const int64_t at = (int64_t)blockIdx.x * (kWarps / p.warps) + warp / p.warps;
+    if (at >= (int64_t)p.c.batch * vh) return;  // (warps of the last block, where p.warps is 1)
+    b = (int)(at / vh);
+    hv = (int)(at % vh);
     s = sequence(p, b);
-    u = (int)((int64_t)s.units * warp / kWarps);
-    todo = (int64_t)s.units * (warp + 1) / kWarps - u;
+    const int part = warp % p.warps;
+    u = s.units * part / p.warps;
+    todo = s.units * (part + 1) / p.warps - u;
   } else {
     int per;
     const int64_t mine = lane_units(p, lane, &per);
@@ -455,38 +470,29 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kerne
     hv = (int)(rest / s.units);
     u = (int)(rest % s.units);
   }
+  if (lane < 2) pieces[warp][lane].bh = -1;
+  __syncwarp();
   Walk<T, D, ROWS> w;
   while (todo > 0) {
     const int u1 = (int)(todo < s.units - u ? u + todo : s.units);
     w.run(p, saddr(ring), lane, b, hv, s, u, u1);
     todo -= u1 - u;
-    // a piece of its own that something follows goes out through `first`, the last one stays here
-    const bool more = todo > 0;
-    if (more && u == 0) {  // whole, and done: finish it
-      w.store(last, lane);
-      __syncwarp();
-      // (one warp joins its only partial)
-      const int h = hv / p.tiles, tile = hv % p.tiles;
-      const int rows = p.G - tile * ROWS < ROWS ? p.G - tile * ROWS : ROWS;
-      for (int e = lane; e < rows * (D / 2); e += 32) {
-        const int r = e / (D / 2), d = e % (D / 2) * 2, head = h * p.G + tile * ROWS + r;
-        const Row f = finish(P::m(last)[r], P::l(last)[r], p.sinks ? p.sinks[head] * kLog2e : -INFINITY);
-        const float2 v = *reinterpret_cast<const float2*>(P::o(last) + r * D + d);
-        *reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.ob + head * p.oh + d) =
-            Pack<T>::pack(v.x * f.inv, v.y * f.inv);
-        if (p.lse && d == 0) p.lse[(int64_t)b * p.Hq + head] = f.lse;
-      }
-      __syncwarp();
+    if (u == 0 && u1 == s.units) {
+      w.write(p, lane, b, hv);
+    } else if (todo > 0) {  // the end of a sequence; the ring is needed again
+      w.store(p.heads + ((int64_t)blockIdx.x * kWarps + warp) * P::kFloats, lane);
+      if (lane == 0) pieces[warp][0] = {b * vh + hv, u, u1, s.units};
     } else {
-      w.store(more ? first : last, lane);
-      if (lane == 0) pieces[warp][more ? 0 : 1] = {b * vh + hv, u, u1, s.units};
+      w.store(reinterpret_cast<float*>(ring), lane);
+      if (lane == 0) pieces[warp][1] = {b * vh + hv, u, u1, s.units};
     }
     u = 0;
-    if (more && ++hv == vh) {
+    if (todo > 0 && ++hv == vh) {
       hv = 0;
       s = sequence(p, ++b);
     }
   }
+  if (p.warps == 1) return;
   __syncthreads();
 
   // join neighbouring pieces of the same (sequence, KV head, tile)
@@ -512,72 +518,178 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kerne
       return x % 2 ? reinterpret_cast<float*>(smem + x / 2 * Shape<D>::kRing)
                    : p.heads + ((int64_t)blockIdx.x * kWarps + x / 2) * P::kFloats;
     };
-    join<T, D, ROWS, kThreads>(p, a.bh / vh, a.bh % vh, count, part, into);
+    join<T, D, ROWS>(p, a.bh / vh, a.bh % vh, count, part, into);
   }
 }
 
-// The sequences that span blocks: a block per (sequence, KV head, tile) finds the blocks that hold
-// it by the same dealing out, and joins their partials.
-template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(DecodeParams p, int grid) {
-  using P = Partial<D, ROWS>;
-  const int lane = threadIdx.x % 32, vh = p.c.n_kv_heads * p.tiles;
-  const int b = blockIdx.x / vh, hv = blockIdx.x % vh;
-  int64_t all = 0, before = 0;
-  for (int i = lane; i < p.c.batch; i += 32) {
-    const int n = sequence(p, i).units;
-    all += n;
-    if (i < b) before += n;
-  }
-  const int64_t total = warp_sum(all) * vh;
-  const int units = sequence(p, b).units, blocks = active_blocks(total, grid);
-  const int64_t start = warp_sum(before) * vh + (int64_t)hv * units, end = start + units;
-  // block c holds [total c / blocks, total (c + 1) / blocks)
-  const int c0 = (int)(((start + 1) * blocks - 1) / total), c1 = (int)((end * blocks - 1) / total);
-  sm100::pdl_wait();
-  if (c0 == c1) return;
-  auto part = [&](int i) -> float* {
-    const int c = c0 + i;
-    const int64_t from = total * c / blocks;
-    return p.partials + ((int64_t)c * 2 + (from > start ? 0 : 1)) * P::kFloats;
-  };
-  join<T, D, ROWS, kJoinThreads>(p, b, hv, c1 - c0 + 1, part, nullptr);
-}
-
-// weights_out = decay * weights + the group's softmax weights, exp2 of the stored scores less the
-// finished log-sum-exp.
-template <int ROWS>
-__global__ void __launch_bounds__(kWeightThreads) weights_kernel(DecodeParams p, int tiles_x) {
-  const int hk = blockIdx.x / tiles_x % p.c.n_kv_heads, b = blockIdx.x / tiles_x / p.c.n_kv_heads;
-  const Sequence s = sequence(p, b);
-  const int slot = blockIdx.x % tiles_x * kWeightThreads + threadIdx.x;
-  if (slot >= s.n) return;
-  float w = p.c.weights ? p.decay * p.c.weights[b * p.c.wb + hk * p.c.wh + slot] : 0.f;
-  sm100::pdl_wait();
-  if (slot < s.sinks || slot >= s.first) {
-    const int chunk = slot / kUnit, u = chunk < s.a ? chunk : chunk - s.c0 + s.a;
-    float sum = 0.f;
-    for (int tile = 0; tile < p.tiles; ++tile) {
-      const int rows = p.G - tile * ROWS < ROWS ? p.G - tile * ROWS : ROWS;
-      const float* sc = p.scores + ((((int64_t)b * p.c.n_kv_heads + hk) * p.tiles + tile) * p.max_units + u) * (ROWS * kUnit) +
-                        slot % kUnit;
-      const float* lse = p.lse + (int64_t)b * p.Hq + hk * p.G + tile * ROWS;
-      for (int r = 0; r < rows; ++r) sum += fast_exp2(sc[r * kUnit] - lse[r]);
+// The blocks of decode_kernel that hold units of (b, hv), found by the same dealing out, and their
+// partials.
+template <int D, int ROWS> struct Span {
+  int c0, c1, blocks;
+  int64_t total, start;
+  float* partials;
+  __device__ __forceinline__ Span(const DecodeParams& p, int b, int hv, int grid) {
+    const int lane = threadIdx.x % 32, vh = p.c.n_kv_heads * p.tiles;
+    int64_t all = 0, before = 0;
+    int units = 0;
+    for (int i = lane; i < p.c.batch; i += 32) {
+      const int n = sequence(p, i).units;
+      all += n;
+      if (i < b) before += n;
+      if (i == b) units = n;
     }
-    w += sum;
+    units = __shfl_sync(~0u, units, b % 32);
+    total = warp_sum(all) * vh;
+    start = warp_sum(before) * vh + (int64_t)hv * units;
+    blocks = active_blocks(total, grid);
+    // block c holds [total c / blocks, total (c + 1) / blocks)
+    c0 = (int)(((start + 1) * blocks - 1) / total);
+    c1 = (int)(((start + units) * blocks - 1) / total);
+    partials = p.partials;
   }
-  p.wout[b * p.wob + hk * p.woh + slot] = w;
+  __device__ __forceinline__ bool split() const { return c1 > c0; }
+  __device__ __forceinline__ float* part(int c) const {
+    return partials + ((int64_t)c * 2 + (c > c0 ? 0 : 1)) * Partial<D, ROWS>::kFloats;
+  }
+};
+
+// Maximum and sum of row r over a span's partials, by one warp.
+template <int D, int ROWS>
+__device__ __forceinline__ void span_stats(const Span<D, ROWS>& s, int r, int lane, float* m, float* l) {
+  using P = Partial<D, ROWS>;
+  float mm = -INFINITY, ll = 0.f;
+  for (int c = s.c0 + lane; c <= s.c1; c += 32) {
+    const float x = P::m(s.part(c))[r], y = P::l(s.part(c))[r], up = fmaxf(mm, x), base = up == -INFINITY ? 0.f : up;
+    ll = ll * fast_exp2(mm - base) + y * fast_exp2(x - base);
+    mm = up;
+  }
+  float top = mm;
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  ll *= fast_exp2(mm - (top == -INFINITY ? 0.f : top));
+  for (int o = 16; o; o >>= 1) ll += __shfl_xor_sync(~0u, ll, o);
+  *m = top;
+  *l = ll;
+}
+
+// After decode_kernel.  Blocks [0, joins): one per (sequence, KV head, tile, row), which joins the
+// row's partials where the sequence spans blocks, each warp every fourth one.  Behind them, with
+// weights_out, blocks of kWeightSlots slots of a (sequence, KV head):
+//   weights_out = decay * weights + sum over the heads of exp2(stored score - log-sum-exp),
+// with the log-sum-exp joined once more where it spans blocks, so that nothing waits for the joins.
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(kThreads) finish_kernel(DecodeParams p, int grid, int joins, int weight_tiles) {
+  using P = Partial<D, ROWS>;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, vh = p.c.n_kv_heads * p.tiles;
+  if ((int)blockIdx.x < joins) {
+    constexpr int V = D >= 32 ? D / 32 : 1;  // values of a lane
+    __shared__ float sums[kWarps][D];
+    const int r = blockIdx.x % ROWS, bh = blockIdx.x / ROWS, b = bh / vh, hv = bh % vh;
+    const int row = hv % p.tiles * ROWS + r, head = hv / p.tiles * p.G + row;
+    if (row >= p.G) {
+      sm100::pdl_wait();  // (every block waits: the grid is not over before the one that it follows)
+      return;
+    }
+    const Span<D, ROWS> s(p, b, hv, grid);
+    const float sink = p.sinks ? p.sinks[head] * kLog2e : -INFINITY;
+    sm100::pdl_wait();
+    if (!s.split()) return;
+    float m, l, acc[V] = {};
+    span_stats(s, r, lane, &m, &l);
+    const float base = m == -INFINITY ? 0.f : m;
+    const bool live = lane * V < D;
+#pragma unroll 8
+    for (int c = s.c0 + warp; c <= s.c1; c += kWarps) {
+      float* q = s.part(c);
+      const float f = fast_exp2(P::m(q)[r] - base);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (live) acc[i] = fmaf(P::o(q)[r * D + lane * V + i], f, acc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (live) sums[warp][lane * V + i] = acc[i];
+    __syncthreads();
+    const Row w = finish(m, l, sink);
+    for (int d = threadIdx.x; d < D; d += kThreads) {
+      float x = 0.f;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) x += sums[i][d];
+      static_cast<T*>(p.o)[b * p.ob + head * p.oh + d] = Pack<T>::from(x * w.inv);
+    }
+    if (p.lse && threadIdx.x == 0) p.lse[(int64_t)b * p.Hq + head] = w.lse;
+    return;
+  }
+  const int at = blockIdx.x - joins, hk = at / weight_tiles % p.c.n_kv_heads, b = at / weight_tiles / p.c.n_kv_heads;
+  const Sequence s = sequence(p, b);
+  const int slot0 = at % weight_tiles * kWeightSlots;
+  if (slot0 >= s.n) {
+    sm100::pdl_wait();
+    return;
+  }
+  constexpr int kPer = kWeightSlots / kThreads;
+  __shared__ float lse[ROWS];
+  float w[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int slot = slot0 + i * kThreads + threadIdx.x;
+    w[i] = slot < s.n && p.c.weights ? p.decay * p.c.weights[b * p.c.wb + hk * p.c.wh + slot] : 0.f;
+  }
+  sm100::pdl_wait();
+  for (int tile = 0; tile < p.tiles; ++tile) {
+    const int hv = hk * p.tiles + tile, rows = p.G - tile * ROWS < ROWS ? p.G - tile * ROWS : ROWS;
+    __syncthreads();
+    if (p.warps) {
+      if ((int)threadIdx.x < rows) lse[threadIdx.x] = p.lse[(int64_t)b * p.Hq + hk * p.G + tile * ROWS + threadIdx.x];
+    } else {
+      const Span<D, ROWS> span(p, b, hv, grid);
+      for (int r = warp; r < rows; r += kWarps) {
+        const int head = hk * p.G + tile * ROWS + r;
+        float m = 0.f, l = 0.f;
+        if (span.split()) span_stats(span, r, lane, &m, &l);
+        if (lane == 0)
+          lse[r] = span.split() ? finish(m, l, p.sinks ? p.sinks[head] * kLog2e : -INFINITY).lse
+                                : p.lse[(int64_t)b * p.Hq + head];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int slot = slot0 + i * kThreads + threadIdx.x;
+      if (slot < s.n && (slot < s.sinks || slot >= s.first)) {
+        const int chunk = slot / kUnit, u = chunk < s.a ? chunk : chunk - s.c0 + s.a;
+        const float4* sc = reinterpret_cast<const float4*>(
+            p.scores + (((int64_t)b * vh + hv) * p.max_units + u) * (ROWS * kUnit) + slot % kUnit * ROWS);
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < ROWS; r += 4) {
+          if (r < rows) {
+            const float4 x = sc[r / 4];
+            sum += fast_exp2(x.x - lse[r]);
+            if (r + 1 < rows) sum += fast_exp2(x.y - lse[r + 1]);
+            if (r + 2 < rows) sum += fast_exp2(x.z - lse[r + 2]);
+            if (r + 3 < rows) sum += fast_exp2(x.w - lse[r + 3]);
+          }
+        }
+        w[i] += sum;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int slot = slot0 + i * kThreads + threadIdx.x;
+    if (slot < s.n) p.wout[b * p.wob + hk * p.woh + slot] = w[i];
+  }
 }
 
 // What a call needs of the workspace, in floats each, every part a multiple of 64.
 struct Plan {
-  int rows, tiles, max_units, whole, blocks;
+  int rows, tiles, max_units, warps, blocks;
   size_t lse, partials, heads, scores;
 };
 size_t round64(size_t n) { return (n + 63) & ~(size_t)63; }
 
-// Visible units from which a sequence is split: below, a block of its own is as quick as a split
-// and saves the join.
+// Visible units from which sequences are dealt out over blocks: below, a block of its own is as
+// quick and saves the join.
 constexpr int kWholeUnits = 32;
 
 Plan plan(const SwaPagedDecodeArgs& a) {
@@ -593,16 +705,20 @@ Plan plan(const SwaPagedDecodeArgs& a) {
   const int64_t bound = ((int64_t)a.sink_size + kUnit - 1) / kUnit + (w + kUnit - 1) / kUnit + 1;
   if (bound < units) units = bound;
   r.max_units = units > 0 ? (int)units : 1;
-  const int64_t vh = (int64_t)c.n_kv_heads * r.tiles, seqs = vh * c.batch;
-  r.whole = r.max_units <= kWholeUnits;
+  const int64_t seqs = (int64_t)c.batch * c.n_kv_heads * r.tiles;
   const int most = D == 128 ? Shape<128>::kMaxBlocks : Shape<64>::kMaxBlocks;
-  // at least two units a warp
-  const int64_t want = (seqs * r.max_units + 2 * kWarps - 1) / (2 * kWarps);
-  r.blocks = (int)(r.whole ? seqs : want < most ? want : most);
+  if (r.max_units <= kWholeUnits) {
+    // a warp each where that fills the GPU: no join, and four times as many in flight
+    r.warps = seqs >= most ? 1 : kWarps;
+    r.blocks = (int)((seqs * r.warps + kWarps - 1) / kWarps);
+  } else {
+    const int64_t want = (seqs * r.max_units + 2 * kWarps - 1) / (2 * kWarps);
+    r.blocks = (int)(want < most ? want : most);
+  }
   const size_t part = (size_t)r.rows * (D + 2);
   r.lse = a.weights_out && !a.lse ? round64((size_t)c.batch * a.n_q_heads) : 0;
-  r.partials = r.whole ? 0 : round64(2 * part * r.blocks);
-  r.heads = r.whole ? 0 : round64(kWarps * part * r.blocks);
+  r.partials = r.warps ? 0 : round64(2 * part * r.blocks);
+  r.heads = r.warps ? 0 : round64(kWarps * part * r.blocks);
   r.scores = a.weights_out ? round64((size_t)seqs * r.max_units * r.rows * kUnit) : 0;
   return r;
 }
@@ -614,15 +730,13 @@ cudaError_t launch(const DecodeParams& p, const Plan& pl, cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   kern<<<pl.blocks, kThreads, smem, st>>>(p);
-  e = cudaGetLastError();
-  const int seqs = p.c.batch * p.c.n_kv_heads * p.tiles;
-  if (e == cudaSuccess && !p.whole)
-    e = launch_pdl(join_kernel<T, D, ROWS>, seqs, kJoinThreads, 0, st, p, pl.blocks);
-  if (e == cudaSuccess && p.wout) {
-    const int x = (p.c.max_pages * p.c.page_size + kWeightThreads - 1) / kWeightThreads;
-    if (x > 0) e = launch_pdl(weights_kernel<ROWS>, x * p.c.n_kv_heads * p.c.batch, kWeightThreads, 0, st, p, x);
-  }
-  return e;
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  const int64_t joins = p.warps ? 0 : (int64_t)p.c.batch * p.c.n_kv_heads * p.tiles * ROWS;
+  const int64_t slots = (int64_t)p.c.max_pages * p.c.page_size;
+  const int64_t tiles = p.wout ? (slots + kWeightSlots - 1) / kWeightSlots : 0;
+  const int64_t blocks = joins + tiles * p.c.n_kv_heads * p.c.batch;
+  if (blocks == 0) return cudaSuccess;
+  return launch_pdl(finish_kernel<T, D, ROWS>, (int)blocks, kThreads, 0, st, p, pl.blocks, (int)joins, (int)tiles);
 }
 
 template <typename T, int ROWS>
@@ -649,7 +763,7 @@ cudaError_t launch_paged_decode(const PagedParams& c, const SwaPagedDecodeArgs& 
   p.Hq = a.n_q_heads; p.G = a.n_q_heads / c.n_kv_heads; p.tiles = pl.tiles;
   p.W = a.window_size; p.S = a.sink_size;
   p.units_per_page = c.page_size / kUnit;
-  p.max_units = pl.max_units; p.whole = pl.whole;
+  p.max_units = pl.max_units; p.warps = pl.warps;
   p.scale_log2 = a.softmax_scale * kLog2e;
   p.q = a.q.ptr; p.o = a.o.ptr;
   p.qb = a.q.stride_t; p.qh = a.q.stride_h; p.ob = a.o.stride_t; p.oh = a.o.stride_h;
