@@ -241,21 +241,38 @@ def check(status: int, where: str):
     raise cls(status, where, detail)
 
 
-class _Same:
-    def __enter__(self):
-        pass
+class Calls:
+    """Argument blocks by what a call's arguments look like (shapes, strides, sizes; no address),
+    so that a call like an earlier one copies a block and fills in addresses instead of checking
+    and building all of it again.  Serving and training repeat few forms; the oldest go first."""
 
-    def __exit__(self, *a):
-        pass
+    def __init__(self, most=256):
+        self._blocks, self._most = {}, most
+
+    def get(self, key):
+        return self._blocks.get(key)
+
+    def put(self, key, block):
+        with _lock:
+            if len(self._blocks) >= self._most:
+                self._blocks.pop(next(iter(self._blocks)))
+            self._blocks[key] = block
+        return block
 
 
-_SAME = _Same()
-
-
-def on_device(dev):
-    """Context in which ``dev`` is the current device (nothing to do where it already is)."""
+def call(name, args, dev):
+    """Call an entry point of the library on ``dev`` and its current stream, raise on a status."""
     import torch
-    return _SAME if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    index = dev.index
+    # the stream's handle without a Stream object around it (3 us of a call's 13)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch.cuda.current_device() == index:
+        status = getattr(lib(), name)(ctypes.byref(args), stream)
+    else:
+        with torch.cuda.device(index):
+            status = getattr(lib(), name)(ctypes.byref(args), stream)
+    if status:
+        check(status, name)
 
 
 # ---------------------------------------------------------------------------------------

@@ -41,6 +41,9 @@ int build_rotary(const SwaRotary& r, int head_dim, bool need_ptrs, swa::RotaryPa
   return SWA_OK;
 }
 
+// Heads share the blocks of one grid dimension.
+bool heads_ok(int64_t q, int64_t kv) { return q + 2 * kv <= 65535; }
+
 bool strides_ok(const SwaTensor& t) { return t.stride_b >= 0 && t.stride_h >= 0 && t.stride_l >= 0; }
 bool packed_ok(const SwaPackedTensor& t) { return t.ptr && t.stride_t >= 0 && t.stride_h >= 0; }
 
@@ -90,6 +93,8 @@ int swa_rotary(const SwaRotaryArgs* a, void* stream) {
   if (a->batch < 0 || a->seq_len < 0 || a->n_q_heads <= 0 || a->n_kv_heads < 0) return SWA_ERR_INVALID_ARG;
   if (a->head_dim <= 0 || a->head_dim > 128 || a->head_dim % 2) return SWA_ERR_INVALID_ARG;
   if (a->dtype != SWA_F16 && a->dtype != SWA_BF16) return SWA_ERR_UNSUPPORTED;
+  if ((int64_t)a->batch * a->seq_len > INT32_MAX / 2 || !heads_ok(a->n_q_heads, a->n_kv_heads))
+    return SWA_ERR_UNSUPPORTED;
   const bool empty = (int64_t)a->batch * a->seq_len == 0;
   swa::RotaryParams r;
   if (int st = build_rotary(a->r, a->head_dim, !empty, &r)) return st;
@@ -106,6 +111,7 @@ int swa_paged_append(const SwaPagedAppendArgs* a, void* stream) {
   swa::PagedParams c;
   if (int st = build_cache(a->cache, &c)) return st;
   if (a->n_tokens < 0 || a->n_q_heads < 0) return SWA_ERR_INVALID_ARG;
+  if (!heads_ok(a->n_q_heads, c.n_kv_heads) || a->n_tokens > INT32_MAX / 2) return SWA_ERR_UNSUPPORTED;
   const bool empty = a->n_tokens == 0 || c.batch == 0;
   swa::RotaryParams r = {};
   if (a->use_rotary)

@@ -727,7 +727,7 @@ template <typename T, int D, int ROWS>
 cudaError_t launch(const DecodeParams& p, const Plan& pl, cudaStream_t st) {
   constexpr int smem = kWarps * Shape<D>::kRing;
   auto kern = decode_kernel<T, D, ROWS>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_smem<Walk<T, D, ROWS>>(kern, smem);
   if (e != cudaSuccess) return e;
   kern<<<pl.blocks, kThreads, smem, st>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;

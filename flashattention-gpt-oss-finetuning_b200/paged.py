@@ -12,8 +12,8 @@ grouped heads.  Keys and values lie in pages of one pool, ``[n_pages, Hkv, page_
 
 With ``weights`` and ``positions`` the cache also tracks how much attention each slot has had
 (``decode(..., weights_out=cache.weights)``), and ``evict`` cuts sequences down to a budget by it.
-All calls are asynchronous on the current stream and can be captured into a CUDA graph.  The
-compute is the C-ABI library's ``swa_paged_append`` / ``swa_paged_decode`` / ``swa_paged_evict``.
+All calls are asynchronous on the current stream and can be captured into a CUDA graph; none is
+differentiable.  The compute is the C-ABI library's ``swa_paged_append`` / ``swa_paged_decode`` / ``swa_paged_evict``.
 """
 from __future__ import annotations
 
@@ -24,7 +24,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .flash_attention_gpt_oss import _DTYPES, _KERNEL_HEAD_DIMS, _stream
+from .flash_attention_gpt_oss import _DTYPES, _KERNEL_HEAD_DIMS
 from .rotary import Rotary
 
 _WHOLE = 2**31 - 1
@@ -32,12 +32,20 @@ _WHOLE = 2**31 - 1
 
 def _rows_ok(t: torch.Tensor) -> bool:
     """Rows of 16-byte aligned, contiguous values."""
-    return t.stride(-1) == 1 and all(s % 8 == 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0
+    *outer, inner = t.stride()
+    bits = t.data_ptr() // 2
+    for s in outer:
+        bits |= s
+    return inner == 1 and bits % 8 == 0
 
 
 def _packed(t: torch.Tensor) -> _lib.SwaPackedTensor:
-    s = t.stride()
-    return _lib.SwaPackedTensor(t.data_ptr(), s[0], s[1])
+    return _lib.SwaPackedTensor(None, *t.stride()[:2])
+
+
+def _form(t: Optional[torch.Tensor]):
+    """All of a tensor but its address and device."""
+    return None if t is None else (t.shape, t.stride(), t.dtype)
 
 
 class PagedKVCache:
@@ -103,7 +111,7 @@ class PagedKVCache:
                                   ptr(page_table), page_table.stride(0), ptr(seq_lens), ptr(seen), ptr(weights),
                                   ptr(positions), *st(weights), *st(positions), n, page, m, b, hkv, d,
                                   _DTYPES[k_pages.dtype])
-        self._plans = {}
+        self._calls = _lib.Calls()
 
     @classmethod
     def allocate(cls, batch: int, n_kv_heads: int, head_dim: int, max_len: int, page_size: int = 64,
@@ -137,8 +145,8 @@ class PagedKVCache:
 
     def check(self):
         """Synchronise, and raise if a call met a page number or a length out of range."""
-        with _lib.on_device(self._dev):
-            _lib.check(_lib.lib().swa_check_device(_stream(self._dev)), "PagedKVCache")
+        with torch.cuda.device(self._dev):
+            _lib.check(_lib.lib().swa_check_device(torch.cuda.current_stream().cuda_stream), "PagedKVCache")
 
     def _tokens(self, name, t, heads=None):
         if t.dim() != 3 or t.shape[-1] != self._d or (heads is not None and t.shape[1] != heads):
@@ -146,8 +154,11 @@ class PagedKVCache:
                              f"got {tuple(t.shape)}")
         if t.dtype != self._dtype:
             raise TypeError(f"{name} must be {self._dtype} like the pages; got {t.dtype}")
-        if t.device != self._dev:
-            raise ValueError(f"{name} must be on the device of the pages")
+
+    def _here(self, *tensors):
+        for t in tensors:
+            if t is not None and t.device != self._dev:
+                raise ValueError("all tensors of a call must be on the device of the pages")
 
     def append(self, k: torch.Tensor, v: torch.Tensor, cu_new: Optional[torch.Tensor] = None,
                q: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
@@ -158,6 +169,31 @@ class PagedKVCache:
         ``[B + 1]`` CUDA offsets of each sequence's tokens; omitted, every sequence has T / B.
         With ``rotary`` and ``positions`` (``[T]``, or ``[axes, T]``), k is rotated on the way, and
         so is ``q`` ``[T, Hq, D]``, which is returned."""
+        k = k if k.stride(-1) == 1 else k.contiguous()
+        v = v if v.stride(-1) == 1 else v.contiguous()
+        if q is not None and q.stride(-1) != 1:
+            q = q.contiguous()
+        key = ("append", rotary, _form(k), _form(v), _form(q), _form(positions), _form(cu_new))
+        block = self._calls.get(key)
+        if block is None:
+            block = self._calls.put(key, self._append_block(k, v, cu_new, q, positions, rotary))
+        self._here(k, v, cu_new, q, positions)
+        args = _lib.SwaPagedAppendArgs.from_buffer_copy(block)
+        args.k.ptr, args.v.ptr = k.data_ptr(), v.data_ptr()
+        if cu_new is not None:
+            args.cu_new = cu_new.data_ptr()
+        out = None
+        if rotary is not None:
+            rotary._on(self._dev, positions)
+            args.r.positions = positions.data_ptr()
+            if q is not None:
+                out = torch.empty(q.shape, device=self._dev, dtype=self._dtype)
+                args.q.ptr, args.q_out.ptr = q.data_ptr(), out.data_ptr()
+        _lib.call("swa_paged_append", args, self._dev)
+        return out
+
+    def _append_block(self, k, v, cu_new, q, positions, rotary) -> _lib.SwaPagedAppendArgs:
+        """The argument block of an append of this form, without addresses."""
         self._tokens("k", k, self._hkv)
         self._tokens("v", v, self._hkv)
         t = k.shape[0]
@@ -168,43 +204,23 @@ class PagedKVCache:
         if cu_new is None:
             if t and (self._b == 0 or t % self._b):
                 raise ValueError(f"{t} tokens cannot be dealt out evenly to {self._b} sequences: give cu_new")
-        elif cu_new.dtype != torch.int32 or cu_new.shape != (self._b + 1,) or cu_new.device != self._dev \
-                or (self._b and cu_new.stride(0) != 1):
-            raise ValueError(f"cu_new must be a contiguous int32 [{self._b + 1}] tensor on the pages' device")
-        k = k if k.stride(-1) == 1 else k.contiguous()
-        v = v if v.stride(-1) == 1 else v.contiguous()
+        elif cu_new.dtype != torch.int32 or cu_new.shape != (self._b + 1,) or (self._b and cu_new.stride(0) != 1):
+            raise ValueError(f"cu_new must be a contiguous int32 [{self._b + 1}] tensor")
         none = _lib.SwaPackedTensor(None, 0, 0)
-        args = _lib.SwaPagedAppendArgs(self._c, None if cu_new is None else cu_new.data_ptr(), t, 0, _packed(k),
-                                       _packed(v), none, none, 0)
-        out = None
+        args = _lib.SwaPagedAppendArgs(self._c, None, t, 0, _packed(k), _packed(v), none, none, 0)
         if rotary is not None:
             if not isinstance(rotary, Rotary):
                 raise TypeError("rotary must be a Rotary")
             if rotary.dim > self._d:
                 raise ValueError(f"rotary turns {rotary.dim} values of a head of {self._d}")
-            args.use_rotary, args.r = 1, rotary._bind(positions, self._dev, None, t)
+            args.use_rotary, args.r = 1, rotary._bind(positions, None, t)
             if q is not None:
                 self._tokens("q", q)
                 if q.shape[0] != t:
                     raise ValueError("q and k must have the same tokens")
-                q = q if q.stride(-1) == 1 else q.contiguous()
-                out = torch.empty(q.shape, device=self._dev, dtype=self._dtype)
-                args.n_q_heads, args.q, args.q_out = q.shape[1], _packed(q), _packed(out)
-        with _lib.on_device(self._dev):
-            _lib.check(_lib.lib().swa_paged_append(ctypes.byref(args), _stream(self._dev)), "swa_paged_append")
-        return out
-
-    def _decode_plan(self, hq: int, window: int, sinks: int, weigh: bool):
-        """Argument block and workspace size for this number of query heads and this mask."""
-        key = (hq, window, sinks, weigh)
-        plan = self._plans.get(key)
-        if plan is None:
-            if hq <= 0 or hq % self._hkv:
-                raise ValueError("Number of query heads must be divisible by number of K/V heads")
-            args = _lib.SwaPagedDecodeArgs(self._c, hq, window, sinks)
-            args.weights_out = 256 if weigh else None  # its size counts, its address not yet
-            plan = self._plans[key] = (args, _lib.lib().swa_paged_decode_workspace_size(ctypes.byref(args)))
-        return plan
+                args.n_q_heads, args.q = q.shape[1], _packed(q)
+                args.q_out = _lib.SwaPackedTensor(None, q.shape[1] * self._d, self._d)
+        return args
 
     def decode(self, q: torch.Tensor, window_size: Optional[int] = None, sink_size: int = 0,
                softmax_scale: Optional[float] = None, sinks: Optional[torch.Tensor] = None,
@@ -217,40 +233,64 @@ class PagedKVCache:
         weights of this token, summed over the query heads of each KV head, in the slots in use
         (``cache.weights`` itself to accumulate in place; without cache.weights only the new ones).
         ``return_lse``: also the base-2 log-sum-exp ``[B, Hq]``."""
-        self._tokens("q", q)
-        if q.shape[0] != self._b:
-            raise ValueError(f"q must hold one token for each of {self._b} sequences; got {q.shape[0]}")
-        hq, dev = q.shape[1], self._dev
-        window = _WHOLE if window_size is None else max(-1, min(int(window_size), _WHOLE))
-        plan, ws_bytes = self._decode_plan(hq, window, min(int(sink_size), _WHOLE), weights_out is not None)
         if not _rows_ok(q):
             q = q.clone(memory_format=torch.contiguous_format)
-        o = torch.empty((self._b, hq, self._d), device=dev, dtype=self._dtype)
-        args = _lib.SwaPagedDecodeArgs.from_buffer_copy(plan)
-        args.softmax_scale = 1.0 / math.sqrt(self._d) if softmax_scale is None else float(softmax_scale)
-        args.q, args.o = _packed(q), _packed(o)
-        lse = torch.empty((self._b, hq), device=dev, dtype=torch.float32) if return_lse else None
-        args.lse = None if lse is None else lse.data_ptr()
+        # numbers as numbers: a tensor's value could change under its key
+        window_size = None if window_size is None else int(window_size)
+        softmax_scale = None if softmax_scale is None else float(softmax_scale)
+        sink_size, decay = int(sink_size), float(decay)
+        key = ("decode", _form(q), window_size, sink_size, softmax_scale, _form(sinks), _form(weights_out), decay)
+        block = self._calls.get(key)
+        if block is None:
+            block = self._calls.put(key, self._decode_block(q, window_size, sink_size, softmax_scale, sinks, weights_out, decay))
+        dev = self._dev
+        self._here(q, sinks, weights_out)
+        block, ws_bytes, sinks_ok = block
+        args = _lib.SwaPagedDecodeArgs.from_buffer_copy(block)
+        o = torch.empty(q.shape, device=dev, dtype=self._dtype)
+        args.q.ptr, args.o.ptr = q.data_ptr(), o.data_ptr()
+        lse = None
+        if return_lse:
+            lse = torch.empty(q.shape[:2], device=dev, dtype=torch.float32)
+            args.lse = lse.data_ptr()
         if sinks is not None:
-            if sinks.dim() != 1 or sinks.numel() != hq or sinks.device != dev:
-                raise ValueError(f"sinks must be [{hq}] logits on the device of q")
-            if sinks.dtype != torch.float32 or not sinks.is_contiguous():
-                sinks = sinks.detach().to(torch.float32).contiguous()
+            sinks = sinks if sinks_ok else sinks.detach().to(torch.float32).contiguous()
             args.sink_logits = sinks.data_ptr()
         if weights_out is not None:
-            if weights_out.shape != (self._b, self._hkv, self._cap) or weights_out.dtype != torch.float32 or \
-                    weights_out.device != dev or (weights_out.numel() and weights_out.stride(-1) != 1):
-                raise ValueError(f"weights_out must be an fp32 [{self._b}, {self._hkv}, {self._cap}] tensor on the "
-                                 "pages' device with the last dimension contiguous")
             args.weights_out = weights_out.data_ptr()
-            args.wo_stride_b, args.wo_stride_h = weights_out.stride()[:2]
-            args.decay = float(decay)
-        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
-        if ws is not None:
+        if ws_bytes:
+            ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
             args.workspace, args.workspace_bytes = ws.data_ptr(), ws_bytes
-        with _lib.on_device(dev):
-            _lib.check(_lib.lib().swa_paged_decode(ctypes.byref(args), _stream(dev)), "swa_paged_decode")
+        _lib.call("swa_paged_decode", args, dev)
         return (o, lse) if return_lse else o
+
+    def _decode_block(self, q, window_size, sink_size, softmax_scale, sinks, weights_out, decay):
+        """The argument block of an attention of this form, without addresses; the bytes of its
+        workspace; whether the sink logits can be read as they are."""
+        self._tokens("q", q)
+        hq = q.shape[1]
+        if q.shape[0] != self._b:
+            raise ValueError(f"q must hold one token for each of {self._b} sequences; got {q.shape[0]}")
+        if hq <= 0 or hq % self._hkv:
+            raise ValueError("Number of query heads must be divisible by number of K/V heads")
+        if sink_size < 0:
+            raise ValueError("sink_size must not be negative")
+        window = _WHOLE if window_size is None else max(-1, min(window_size, _WHOLE))
+        scale = 1.0 / math.sqrt(self._d) if softmax_scale is None else softmax_scale
+        args = _lib.SwaPagedDecodeArgs(self._c, hq, window, min(sink_size, _WHOLE), scale, _packed(q),
+                                       _lib.SwaPackedTensor(None, hq * self._d, self._d))
+        args.decay = decay
+        if sinks is not None and (sinks.dim() != 1 or sinks.numel() != hq):
+            raise ValueError(f"sinks must be [{hq}] logits")
+        if weights_out is not None:
+            if weights_out.shape != (self._b, self._hkv, self._cap) or weights_out.dtype != torch.float32 or \
+                    (weights_out.numel() and weights_out.stride(-1) != 1):
+                raise ValueError(f"weights_out must be an fp32 [{self._b}, {self._hkv}, {self._cap}] tensor "
+                                 "with the last dimension contiguous")
+            args.weights_out = 256  # it counts for the workspace
+            args.wo_stride_b, args.wo_stride_h = weights_out.stride()[:2]
+        return (args, _lib.lib().swa_paged_decode_workspace_size(ctypes.byref(args)),
+                sinks is not None and sinks.dtype == torch.float32 and sinks.is_contiguous())
 
     def evict(self, keep: int, sink_size: int = 0, recent: int = 0, trigger: Optional[int] = None):
         """Cut sequences of more than ``max(trigger, keep)`` slots down to ``keep``.
@@ -260,19 +300,28 @@ class PagedKVCache:
         where they are, and the others, in order, fill the places that came free, so the order of
         slots is no longer that of tokens: attend with ``window_size=None`` afterwards.
         ``seq_lens`` becomes ``keep``.  Pages of a sequence that is cut must be its own."""
+        keep, sink_size, recent = int(keep), int(sink_size), int(recent)
+        trigger = keep if trigger is None else int(trigger)
+        key = ("evict", keep, sink_size, recent, trigger)
+        block = self._calls.get(key)
+        if block is None:
+            block = self._calls.put(key, self._evict_block(keep, sink_size, recent, trigger))
+        block, ws_bytes = block
+        if block is None:
+            return
+        args = _lib.SwaPagedEvictArgs.from_buffer_copy(block)
+        ws = torch.empty(ws_bytes, device=self._dev, dtype=torch.uint8)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), ws_bytes
+        _lib.call("swa_paged_evict", args, self._dev)
+
+    def _evict_block(self, keep, sink_size, recent, trigger):
+        """The argument block of an eviction (None: no sequence can be that long) and the bytes of
+        its workspace."""
         if self.weights is None or self.positions is None:
             raise ValueError("eviction needs a cache with weights and positions")
-        keep = int(keep)
-        trigger = keep if trigger is None else int(trigger)
         if keep <= 0 or trigger < 0 or sink_size < 0 or recent < 0 or sink_size + recent > keep:
             raise ValueError("keep must be positive and hold sink_size + recent tokens")
-        keep, trigger = min(keep, _WHOLE), min(trigger, _WHOLE)
-        if keep >= self._cap:
-            return
-        args = _lib.SwaPagedEvictArgs(self._c, keep, trigger, int(sink_size), int(recent), None, 0)
-        lib = _lib.lib()
-        n = lib.swa_paged_evict_workspace_size(ctypes.byref(args))
-        ws = torch.empty(max(n, 1), device=self._dev, dtype=torch.uint8)
-        args.workspace, args.workspace_bytes = ws.data_ptr(), n
-        with _lib.on_device(self._dev):
-            _lib.check(lib.swa_paged_evict(ctypes.byref(args), _stream(self._dev)), "swa_paged_evict")
+        if keep >= self._cap or self._b == 0:
+            return None, 0
+        args = _lib.SwaPagedEvictArgs(self._c, keep, min(trigger, _WHOLE), sink_size, recent)
+        return args, _lib.lib().swa_paged_evict_workspace_size(ctypes.byref(args))

@@ -15,7 +15,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from .flash_attention_gpt_oss import _DTYPES, _stream
+from .flash_attention_gpt_oss import _DTYPES
 
 
 class Rotary:
@@ -53,40 +53,43 @@ class Rotary:
             raise ValueError("at most 256 axes")
         if not float(scale) == float(scale):
             raise ValueError("scale is NaN")
-        self.inv_freq = inv_freq.detach().to(torch.float32, copy=True).contiguous()
-        self.n_axes = n_axes
-        self.dim = 2 * n
-        self.interleaved = bool(interleaved)
-        self.scale = float(scale)
-        self._c = _lib.SwaRotary(self.inv_freq.data_ptr(), None, 0, 0, 0, 0, n_axes, n,
-                                 int(self.interleaved), self.scale)
+        self._inv_freq = inv_freq.detach().to(torch.float32, copy=True).contiguous()
+        self._c = _lib.SwaRotary(self._inv_freq.data_ptr(), None, 0, 0, 0, 0, n_axes, n,
+                                 int(bool(interleaved)), float(scale))
         self._c.axis[:n] = axes
+        self._dev = self._inv_freq.device
+        self._calls = _lib.Calls()
 
-    def _bind(self, positions: torch.Tensor, dev: torch.device, batch: Optional[int], length: int) -> _lib.SwaRotary:
-        """The C block for these positions: ``[L]``, ``[B, L]`` or ``[A, ..., L]``; ``batch`` None:
-        packed tokens."""
+    inv_freq = property(lambda self: self._inv_freq)
+    n_axes = property(lambda self: self._c.n_axes)
+    dim = property(lambda self: 2 * self._c.n_freq, doc="values of a head that turn")
+    interleaved = property(lambda self: bool(self._c.interleaved))
+    scale = property(lambda self: self._c.scale)
+
+    def _bind(self, positions: torch.Tensor, batch: Optional[int], length: int) -> _lib.SwaRotary:
+        """The C block for positions of this form (their address is left out): ``[L]``, ``[B, L]``
+        or ``[A, ..., L]``; ``batch`` None: packed tokens."""
         if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
             raise TypeError("positions must be an int32 or int64 tensor")
-        if positions.device != dev or self.inv_freq.device != dev:
-            raise ValueError("positions and inv_freq must be on the device of q")
         shape, st = tuple(positions.shape), positions.stride()
         axis = self.n_axes > 1 or len(shape) == (2 if batch is None else 3)
-        want = ((self.n_axes,) if axis else ())
         rest, rst = (shape[1:], st[1:]) if axis else (shape, st)
-        ok = bool(shape) and shape[:len(want)] == want
+        ok = not axis or shape[:1] == (self.n_axes,)
+        sb = 0
         if batch is not None and len(rest) == 2:
             ok, sb, rest, rst = ok and rest[0] == batch, rst[0], rest[1:], rst[1:]
-        else:
-            sb = 0
         if not ok or rest != (length,):
             raise ValueError(f"positions {shape} do not fit {self.n_axes} axes and "
                              + (f"[{batch}, {length}] tokens" if batch is not None else f"{length} tokens"))
         c = _lib.SwaRotary.from_buffer_copy(self._c)
-        c.positions = positions.data_ptr()
         c.pos_stride_axis = st[0] if axis else 0
         c.pos_stride_b, c.pos_stride_l = sb, rst[0]
         c.pos_is_64 = int(positions.dtype == torch.int64)
         return c
+
+    def _on(self, dev: torch.device, positions: torch.Tensor):
+        if positions.device != dev or self._dev != dev:
+            raise ValueError("positions and inv_freq must be on the device of q")
 
 
 def _as4(t: torch.Tensor) -> torch.Tensor:
@@ -95,13 +98,14 @@ def _as4(t: torch.Tensor) -> torch.Tensor:
 
 
 def _tensor(t: torch.Tensor) -> _lib.SwaTensor:
-    s = t.stride()
-    return _lib.SwaTensor(t.data_ptr(), s[0], s[1], s[2])
+    return _lib.SwaTensor(None, *t.stride()[:3])
+
+
+def _empty(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _validate(q, k, rotary):
-    if not isinstance(rotary, Rotary):
-        raise TypeError("rotary must be a Rotary")
     for name, t in (("q", q), ("k", k)):
         if t is None:
             continue
@@ -109,8 +113,6 @@ def _validate(q, k, rotary):
             raise ValueError("q and k must both be [B, H, L, D] or both be packed [T, H, D]")
         if t.dtype not in _DTYPES or t.dtype != q.dtype:
             raise TypeError(f"q and k must share one dtype in (float16, bfloat16); got {name}: {t.dtype}")
-        if not t.is_cuda or t.device != q.device:
-            raise ValueError("q and k must be on the same CUDA device")
     d = q.shape[-1]
     if d > 128 or d % 2 or d < rotary.dim:
         raise ValueError(f"head dimension {d} must be even, at most 128 and at least {rotary.dim}")
@@ -120,27 +122,46 @@ def _validate(q, k, rotary):
             raise ValueError("q and k must have the same tokens and head dimension")
 
 
+def _block(q, k, positions, rotary, inverse) -> _lib.SwaRotaryArgs:
+    """The argument block of a call of this form, without addresses."""
+    _validate(q, k, rotary)
+    packed = q.dim() == 3
+    b, hq, l, d = _as4(q).shape
+    none = _lib.SwaTensor(None, 0, 0, 0)
+    dense = lambda t: _tensor(_as4(torch.empty(t.shape, device="meta")))  # noqa: E731
+    return _lib.SwaRotaryArgs(b, hq, 0 if k is None else _as4(k).shape[1], l, d, _DTYPES[q.dtype], int(inverse),
+                              rotary._bind(positions, None if packed else b, l), _tensor(_as4(q)),
+                              none if k is None else _tensor(_as4(k)), dense(q), none if k is None else dense(k))
+
+
 def rotate(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, rotary: Rotary,
            inverse: bool = False):
     """``(q', k')`` as new tensors (``k`` and ``k'`` may be None); ``inverse`` turns back, which
     is the gradient of the inputs from the gradient of the outputs.  No autograd."""
-    _validate(q, k, rotary)
-    packed = q.dim() == 3
-    q4 = _as4(q if q.stride(-1) == 1 else q.contiguous())
-    b, hq, l, d = q4.shape
-    r = rotary._bind(positions, q.device, None if packed else b, l)
-    qo = torch.empty_like(q, memory_format=torch.contiguous_format)
-    none = _lib.SwaTensor(None, 0, 0, 0)
-    ko, kt, kot, hkv = None, none, none, 0
+    if not isinstance(rotary, Rotary):
+        raise TypeError("rotary must be a Rotary")
+    if q.stride(-1) != 1:
+        q = q.contiguous()
+    if k is not None and k.stride(-1) != 1:
+        k = k.contiguous()
+    key = (q.shape, q.stride(), q.dtype, None if k is None else (k.shape, k.stride(), k.dtype), positions.shape,
+           positions.stride(), positions.dtype, inverse)
+    block = rotary._calls.get(key)
+    if block is None:
+        block = rotary._calls.put(key, _block(q, k, positions, rotary, inverse))
+    dev = q.device
+    if not q.is_cuda or (k is not None and k.device != dev):
+        raise ValueError("q and k must be on the same CUDA device")
+    rotary._on(dev, positions)
+    args = _lib.SwaRotaryArgs.from_buffer_copy(block)
+    qo = _empty(q)
+    args.q.ptr, args.q_out.ptr, args.r.positions = q.data_ptr(), qo.data_ptr(), positions.data_ptr()
+    ko = None
     if k is not None:
-        k4 = _as4(k if k.stride(-1) == 1 else k.contiguous())
-        ko = torch.empty_like(k, memory_format=torch.contiguous_format)
-        kt, kot, hkv = _tensor(k4), _tensor(_as4(ko)), k4.shape[1]
-    if hq:
-        args = _lib.SwaRotaryArgs(b, hq, hkv, l, d, _DTYPES[q.dtype], int(inverse), r, _tensor(q4), kt,
-                                  _tensor(_as4(qo)), kot)
-        with _lib.on_device(q.device):
-            _lib.check(_lib.lib().swa_rotary(ctypes.byref(args), _stream(q.device)), "swa_rotary")
+        ko = _empty(k)
+        args.k.ptr, args.k_out.ptr = k.data_ptr(), ko.data_ptr()
+    if args.n_q_heads:
+        _lib.call("swa_rotary", args, dev)
     return qo, ko
 
 
@@ -156,7 +177,9 @@ class _Rotate(torch.autograd.Function):
         (positions,) = ctx.saved_tensors
         dq = dq.to(ctx.dtype)
         dk = None if dk is None else dk.to(ctx.dtype)
-        dq, dk = _Rotate.apply(dq, dk, positions, ctx.rotary, not ctx.inverse)
+        # (the gradient of a gradient: only where one is asked for)
+        turn = _Rotate.apply if torch.is_grad_enabled() else rotate
+        dq, dk = turn(dq, dk, positions, ctx.rotary, not ctx.inverse)
         return dq, dk, None, None, None
 
 

@@ -172,8 +172,10 @@ def test_in_place_through_the_library():
     y = x.to(DEV)
     p = pos[0].to(DEV)
     t = R._tensor(y)
+    t.ptr = y.data_ptr()
     none = L.SwaTensor(None, 0, 0, 0)
-    args = L.SwaRotaryArgs(2, 4, 0, 50, 64, L.SWA_F16, 0, rot._bind(p, DEV, 2, 50), t, none, t, none)
+    args = L.SwaRotaryArgs(2, 4, 0, 50, 64, L.SWA_F16, 0, rot._bind(p, 2, 50), t, none, t, none)
+    args.r.positions = p.data_ptr()
     assert L.lib().swa_rotary(ctypes.byref(args), torch.cuda.current_stream().cuda_stream) == 0
     check(x, y, pos[:, :, None], inv, [0] * 32, False, 1.0)
 
