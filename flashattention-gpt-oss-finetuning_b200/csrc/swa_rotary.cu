@@ -13,7 +13,7 @@
 // writes, so outputs may lie on their inputs.
 //
 // Measured on a B200 (6.56 TB/s copy): q and k of the GPT-OSS layer (4 x 72 heads x 4096 x 64, 302
-// MB moved) 54 us, 5.6 TB/s; 8 x 36 heads x 3000 x 128 (443 MB) 76 us, 5.8 TB/s; 14006 packed
+// MB moved) 54 us, 5.6 TB/s; 8 x 36 heads x 3000 x 128 (443 MB) 76 us, 5.8 TB/s; 14004 packed
 // prompt tokens into pages (288 MB) 57 us, 5.1 TB/s; 64 single tokens 4 us.
 #include "swa_host.cuh"
 #include "swa_paged.cuh"
