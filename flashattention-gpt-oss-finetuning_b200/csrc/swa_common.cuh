@@ -258,10 +258,10 @@ __device__ __forceinline__ float fast_exp2(float x) {
 // kernel in the stream drains (every kernel launched this way calls pdl_wait before touching
 // memory that an earlier launch writes).
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_pdl(void (*kern)(KArgs...), int grid, int block, int smem, cudaStream_t st,
+inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, int block, int smem, cudaStream_t st,
                               Args&&... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3((unsigned)block);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = st;

@@ -2,16 +2,17 @@
 // attention has laid on each slot.
 //
 // Each slot has a 32-bit key: held tokens the largest, then the weights in order.  The budget-th
-// largest key t is found digit by digit (11, 11 and 10 bits) from histograms; slots above t are
+// largest key t is found digit by digit, 8 bits at a time, from histograms; slots above t are
 // kept, and of those equal to t the lowest.  Slots that come free below the budget and kept slots
 // behind it are numbered in order, and the i-th of the one takes the i-th of the other: no row is
 // both read and written, so all of them move at once, and only as many as have to.
 //
-// A (sequence, KV head) belongs to a cluster of 1 to 8 blocks, each with a stretch of the slots,
-// whose keys it keeps in shared memory: the weights and token numbers are read once (8 bytes a slot).
-// Histograms and counts of the other blocks are read through distributed shared memory, one
-// cluster barrier a digit.  What bounds it: the dependent steps (load, three digits, two counts)
-// for small caches, the moved rows (2 x 4 D bytes each) for large ones.
+// select_kernel: a (sequence, KV head) belongs to a cluster of 1 to 8 blocks, each with a stretch of
+// the slots, whose keys it keeps in shared memory: the weights and token numbers are read once (8
+// bytes a slot).  Blocks send one another their histograms and counts through distributed shared
+// memory, one cluster barrier a digit.  move_kernel: a thread per 16 bytes of K and of V of a row
+// that moves, and the lengths.  What bounds the first are its dependent steps (load, four digits, two
+// counts), the second the rows, 128 or 256 scattered bytes each.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -27,16 +28,21 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 2048;
+constexpr int kBins = 256;
+constexpr int kDigits = 4;
 constexpr int kMaxCluster = 8;
-constexpr int kMaxKeys = 40960;  // keys a block keeps (160 KB); more are read again from memory
-constexpr int kMoves = 4;        // 16-byte pieces of K and V that a thread has under way
+constexpr int kMaxKeys = 24576;  // keys a block keeps (96 KB, two blocks an SM); more are read again from memory
+constexpr int kAhead = 8;        // slots whose loads a thread has under way
+constexpr int kMoveThreads = 256;
+constexpr int kMoves = 2;        // pieces of a thread of move_kernel
 
 struct EvictParams {
   PagedParams c;
   int keep, trigger, sink, recent;
   int pieces, piece_bits;  // 16-byte pieces of a row, a power of two
-  int32_t* lists;  // [batch, Hkv, 2, keep]: free slots, then the slots that fill them
+  int32_t* counts;  // [batch, Hkv]: moves, -1 where the sequence is not cut
+  int32_t* lists;   // [batch, Hkv, 2, most]: free slots, then the slots that fill them
+  int most;         // moves that a (sequence, KV head) can have
 };
 
 // Order-preserving map of a weight to [0x007fffff, 0xff800000]: NaN as -inf, -0 as +0.
@@ -58,16 +64,16 @@ __device__ __forceinline__ int warp_before(int x, int lane) {
 }
 
 struct Shared {
-  uint32_t hist[3][kBins];
-  int warp[kWarps][2];   // counts of each warp
-  int block[3][2];       // this block's counts, by round
-  int found[3][3];       // digit, slots above it, slots in it
-  int sums[kWarps];
-  int last_equal;
+  uint32_t hist[kDigits][kBins];
+  uint32_t sent[2][kMaxCluster][kBins];  // the blocks' histograms, of even and odd digits
+  int warp[kWarps][2];                   // counts of each warp
+  int block[2][kMaxCluster][2];          // the blocks' counts, by round
+  int found[kDigits][3]; // digit, slots above it, slots in it
+  int last_equal;                        // the last slot with key t that is kept
 };
 
 template <bool KEEP_KEYS>
-__global__ void __launch_bounds__(kThreads) evict_kernel(const __grid_constant__ EvictParams p, int cluster) {
+__global__ void __launch_bounds__(kThreads, 2) select_kernel(const __grid_constant__ EvictParams p, int cluster) {
   extern __shared__ uint32_t keys[];
   __shared__ __align__(16) Shared sh;
   cg::cluster_group cl = cg::this_cluster();
@@ -76,8 +82,14 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const __grid_constant__
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   bool bad = false;
   const int n = paged_len(p.c, b, &bad);
-  if (bad && tid == 0) *p.c.page_error = 1;
-  if (bad || n <= p.keep || n <= p.trigger) return;  // alike for the cluster
+  sm100::pdl_trigger();
+  if (bad || n <= p.keep || n <= p.trigger) {  // alike for the cluster
+    if (tid == 0 && rank == 0) {
+      p.counts[at] = -1;
+      if (bad) *p.c.page_error = 1;
+    }
+    return;
+  }
   // this block's slots [lo, hi), a warp's [wlo, whi)
   const int per = (n + cluster * kThreads - 1) / (cluster * kThreads) * kThreads;
   const int lo = rank * per;
@@ -86,71 +98,91 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const __grid_constant__
   const float* w = p.c.weights + b * p.c.wb + h * p.c.wh;
   const int32_t* pos = p.c.positions + b * p.c.pb + h * p.c.ph;
   const int64_t late = (int64_t)p.c.seen[b] - p.recent;
-  auto read_key = [&](int s) -> uint32_t {
-    const int x = pos[s];
-    return x < p.sink || x >= late ? 0xffffffffu : weight_key(w[s]);
-  };
-  auto key_of = [&](int s) -> uint32_t { return KEEP_KEYS ? keys[s - lo] : read_key(s); };
+  auto make_key = [&](float weight, int x) -> uint32_t { return x < p.sink || x >= late ? 0xffffffffu : weight_key(weight); };
+  auto key_of = [&](int s) -> uint32_t { return KEEP_KEYS ? keys[s - lo] : make_key(w[s], pos[s]); };
 
-  for (int i = tid; i < 3 * kBins; i += kThreads) (&sh.hist[0][0])[i] = 0;
+  for (int i = tid; i < kDigits * kBins; i += kThreads) (&sh.hist[0][0])[i] = 0;
+  if (cluster > 1) cl.barrier_arrive();  // waited for before the first write to another block
   __syncthreads();
   // digits from the top; `prefix` holds those found
   uint32_t prefix = 0;
   int need = p.keep, equal = 0;
 #pragma unroll
-  for (int round = 0; round < 3; ++round) {
-    constexpr int kShift[3] = {21, 10, 0}, kBits[3] = {11, 11, 10};
-    const int shift = kShift[round], bins = 1 << kBits[round];
+  for (int round = 0; round < kDigits; ++round) {
+    const int shift = 24 - 8 * round;
     uint32_t* hist = sh.hist[round];
-#pragma unroll 4
-    for (int base = wlo; base < whi; base += 32) {
-      const int s = base + lane;
-      const bool in = s < whi;
-      uint32_t key = 0;
-      if (in) {
-        if (round == 0) {
-          key = read_key(s);
-          if (KEEP_KEYS) keys[s - lo] = key;
-        } else {
-          key = key_of(s);
+    // one addition for the lanes with the same digit: weights lie in few octaves, held tokens and
+    // weights of 0 in one place
+    auto count = [&](bool counts, uint32_t key) {
+      const uint32_t digit = counts ? (key >> shift) & (kBins - 1) : kBins;
+      const unsigned alike = __match_any_sync(~0u, digit);
+      if (counts && lane == __ffs(alike) - 1) atomicAdd(&hist[digit], (uint32_t)__popc(alike));
+    };
+    if (round == 0) {
+      for (int base = wlo; base < whi; base += 32 * kAhead) {
+        float weight[kAhead];
+        int x[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int s = base + 32 * i + lane;
+          weight[i] = s < whi ? w[s] : 0.f;
+          x[i] = s < whi ? pos[s] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int s = base + 32 * i + lane;
+          const uint32_t key = make_key(weight[i], x[i]);
+          if (KEEP_KEYS && s < whi) keys[s - lo] = key;
+          if (base + 32 * i < whi) count(s < whi, key);
         }
       }
-      const bool counts = in && (round == 0 || (key >> (shift + kBits[round])) == prefix);
-      const uint32_t digit = (key >> shift) & (bins - 1);
-      // runs of one digit (held tokens, weights of 0) as one addition
-      int alike;
-      __match_all_sync(~0u, counts ? digit : 0xffffffffu, &alike);
-      if (alike) {
-        if (counts && lane == 0) atomicAdd(&hist[digit], 32u);
-      } else if (counts) {
-        atomicAdd(&hist[digit], 1u);
+    } else {
+      for (int base = wlo; base < whi; base += 32) {
+        const int s = base + lane;
+        const uint32_t key = s < whi ? key_of(s) : 0u;
+        const bool counts = s < whi && key >> (shift + 8) == prefix;
+        if (__any_sync(~0u, counts)) count(counts, key);
       }
     }
-    if (cluster > 1) cl.sync(); else __syncthreads();
-    // each thread four bins, from the top: bins - 4 tid - 4 ...
-    const int own = bins - 4 * tid - 4;
-    uint4 sum = make_uint4(0, 0, 0, 0);
-    if (own >= 0)
-      for (int r = 0; r < cluster; ++r) {
-        const uint32_t* other = cluster > 1 ? cl.map_shared_rank(hist, r) : hist;
-        const uint4 x = *reinterpret_cast<const uint4*>(other + own);
-        sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
-      }
-    const int mine = (int)(sum.x + sum.y + sum.z + sum.w);
-    int above = warp_before(mine, lane);
-    if (lane == 31) sh.sums[warp] = above + mine;
     __syncthreads();
-    for (int i = 0; i < warp; ++i) above += sh.sums[i];
-    if (above < need && above + mine >= need) {
-      const int c[4] = {(int)sum.w, (int)sum.z, (int)sum.y, (int)sum.x};
-      int i = 0;
-      while (above + c[i] < need) above += c[i++];
-      sh.found[round][0] = own + 3 - i;
-      sh.found[round][1] = above;
-      sh.found[round][2] = c[i];
+    if (cluster > 1) {
+      // 16 bytes of the histogram to a block by each thread
+      const int to = tid / (kBins / 4), part = tid % (kBins / 4);
+      if (round == 0) cl.barrier_wait();
+      if (to < cluster)
+        *cl.map_shared_rank(reinterpret_cast<uint4*>(sh.sent[round & 1][rank]) + part, to) =
+            reinterpret_cast<const uint4*>(hist)[part];
+      cl.sync();
+    }
+    if (warp == 0) {
+      // eight bins a lane, from the top
+      const int own = kBins - 8 * lane - 8;
+      int c[8] = {};
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r) {
+        if (r >= cluster) break;
+        const uint32_t* other = cluster > 1 ? sh.sent[round & 1][r] : hist;
+        const uint4 x = *reinterpret_cast<const uint4*>(other + own), y = *reinterpret_cast<const uint4*>(other + own + 4);
+        c[0] += y.w; c[1] += y.z; c[2] += y.y; c[3] += y.x; c[4] += x.w; c[5] += x.z; c[6] += x.y; c[7] += x.x;
+      }
+      int mine = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mine += c[i];
+      int above = warp_before(mine, lane);
+      if (above < need && above + mine >= need) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (above < need && above + c[i] >= need) {
+            sh.found[round][0] = own + 7 - i;
+            sh.found[round][1] = above;
+            sh.found[round][2] = c[i];
+          }
+          above += c[i];
+        }
+      }
     }
     __syncthreads();
-    prefix = prefix << kBits[round] | (uint32_t)sh.found[round][0];
+    prefix = prefix << 8 | (uint32_t)sh.found[round][0];
     need -= sh.found[round][1];
     equal = sh.found[round][2];
   }
@@ -167,12 +199,15 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const __grid_constant__
       ty += sh.warp[i][1];
     }
     if (cluster > 1) {
-      if (tid == 0) sh.block[round][0] = tx, sh.block[round][1] = ty;
+      if (tid < cluster) {
+        int* o = cl.map_shared_rank(&sh.block[round][rank][0], tid);
+        o[0] = tx;
+        o[1] = ty;
+      }
       cl.sync();
       for (int r = 0; r < rank; ++r) {
-        const int* o = cl.map_shared_rank(&sh.block[round][0], r);
-        ax += o[0];
-        ay += o[1];
+        ax += sh.block[round][r][0];
+        ay += sh.block[round][r][1];
       }
     }
     *bx = ax;
@@ -187,25 +222,21 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const __grid_constant__
       const int s = base + lane;
       x += __popc(__ballot_sync(~0u, s < whi && key_of(s) == t));
     }
-    if (tid == 0) sh.last_equal = -1;
     offsets(0, x, 0, &before, &unused);
-    if (before < need && before + x >= need) {
+    if (before < need && before + x >= need) {  // one warp of the cluster
       for (int base = wlo; base < whi; base += 32) {
         const int s = base + lane;
         const unsigned votes = __ballot_sync(~0u, s < whi && key_of(s) == t);
         if (before + __popc(votes) >= need) {
-          if (votes >> lane & 1 && before + __popc(votes & ((1u << lane) - 1)) + 1 == need) sh.last_equal = s;
+          if (votes >> lane & 1 && before + __popc(votes & ((1u << lane) - 1)) + 1 == need)
+            for (int r = 0; r < cluster; ++r) *(cluster > 1 ? cl.map_shared_rank(&sh.last_equal, r) : &sh.last_equal) = s;
           break;
         }
         before += __popc(votes);
       }
     }
     if (cluster > 1) cl.sync(); else __syncthreads();
-    for (int r = 0; r < cluster; ++r) {
-      const int x = *(cluster > 1 ? cl.map_shared_rank(&sh.last_equal, r) : &sh.last_equal);
-      if (x >= 0) last_equal = x;
-    }
-    __syncthreads();
+    last_equal = sh.last_equal;
   }
   auto kept = [&](int s) -> bool {
     const uint32_t key = key_of(s);
@@ -220,8 +251,8 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const __grid_constant__
     n_move += __popc(votes & ~below);
   }
   offsets(1, n_free, n_move, &free0, &move0);
-  int32_t* free_list = p.lists + (int64_t)at * 2 * p.keep;
-  int32_t* move_list = free_list + p.keep;
+  int32_t* free_list = p.lists + (int64_t)at * 2 * p.most;
+  int32_t* move_list = free_list + p.most;
   for (int base = wlo; base < whi; base += 32) {
     const int s = base + lane;
     const bool one = s < whi && kept(s) != (s < p.keep);
@@ -233,34 +264,40 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const __grid_constant__
     free0 += __popc(votes & below);
     move0 += __popc(votes & ~below);
   }
-  // all moves: the last block's last warp ends at their number
-  if (warp == kWarps - 1 && lane == 0) sh.block[2][0] = move0;
-  __threadfence();
-  if (cluster > 1) cl.sync(); else __syncthreads();
-  const int moves = *(cluster > 1 ? cl.map_shared_rank(&sh.block[2][0], cluster - 1) : &sh.block[2][0]);
+  // the last block's last warp ends at their number
+  if (rank == cluster - 1 && warp == kWarps - 1 && lane == 0) p.counts[at] = move0;
+}
 
-  // 16 bytes of K and of V a thread, neighbouring pieces by neighbouring threads
-  const int64_t all = (int64_t)moves * p.pieces;
-  const int stride = cluster * kThreads;
-  for (int64_t e0 = rank * kThreads + tid; e0 < all; e0 += stride * kMoves) {
+// blockIdx.y strides over (sequence, KV head), blockIdx.x over its moves; then the lengths.
+__global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ EvictParams p) {
+  sm100::pdl_wait();
+  bool bad = false;
+  const int heads = p.c.batch * p.c.n_kv_heads;
+  for (int at = blockIdx.y; at < heads; at += gridDim.y) {
+    const int h = at % p.c.n_kv_heads, b = at / p.c.n_kv_heads, moves = p.counts[at];
+    if (moves >= 0 && h == 0 && blockIdx.x == 0 && threadIdx.x == 0) p.c.seq_lens[b] = p.keep;
+    const int64_t all = (int64_t)moves * p.pieces;
+    const int32_t* free_list = p.lists + (int64_t)at * 2 * p.most;
+    const int32_t* move_list = free_list + p.most;
+    const int64_t e0 = (int64_t)blockIdx.x * kMoveThreads * kMoves + threadIdx.x;
     uint4 kx[kMoves], vx[kMoves];
     char *kd[kMoves], *vd[kMoves];
     bool ok[kMoves];
 #pragma unroll
     for (int i = 0; i < kMoves; ++i) {
-      const int64_t e = e0 + i * stride;
+      const int64_t e = e0 + i * kMoveThreads;
       ok[i] = e < all;
       if (ok[i]) {
         const int m = (int)(e >> p.piece_bits), part = (int)e & (p.pieces - 1);
         const int to = free_list[m], from = move_list[m];
         const int pt = paged_page(p.c, b, to / p.c.page_size, &bad), pf = paged_page(p.c, b, from / p.c.page_size, &bad);
-        ok[i] = pt >= 0 && pf >= 0;
         if (part == 0) {
-          float* wr = p.c.weights + b * p.c.wb + h * p.c.wh;
-          int32_t* pr = p.c.positions + b * p.c.pb + h * p.c.ph;
-          wr[to] = wr[from];
-          pr[to] = pr[from];
+          float* w = p.c.weights + b * p.c.wb + h * p.c.wh;
+          int32_t* x = p.c.positions + b * p.c.pb + h * p.c.ph;
+          w[to] = w[from];
+          x[to] = x[from];
         }
+        ok[i] = pt >= 0 && pf >= 0;
         if (ok[i]) {
           char* k = static_cast<char*>(p.c.k) + 2 * h * p.c.kh + 16 * part;
           char* v = static_cast<char*>(p.c.v) + 2 * h * p.c.vh + 16 * part;
@@ -280,30 +317,20 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const __grid_constant__
       }
   }
   if (bad) *p.c.page_error = 1;
-  if (cluster > 1) cl.sync();  // nobody leaves while its count is read
 }
 
-// The lengths, once every head has read the old ones.
-__global__ void evict_lens_kernel(PagedParams c, int keep, int trigger) {
-  sm100::pdl_wait();
-  const int b = blockIdx.x * blockDim.x + threadIdx.x;
-  if (b >= c.batch) return;
-  bool bad = false;
-  const int n = paged_len(c, b, &bad);
-  if (!bad && n > keep && n > trigger) c.seq_lens[b] = keep;
-}
-
-// Blocks per (sequence, KV head): as few as give every SM two, or each block no more than 2048 slots.
+// Blocks per (sequence, KV head): as many as fit beside one another (two an SM), of no less than
+// 2048 slots each; more where a block could not keep its keys.
 int cluster_size(const PagedParams& c) {
   const int64_t heads = (int64_t)c.batch * c.n_kv_heads, slots = (int64_t)c.max_pages * c.page_size;
   int size = 1;
-  while (size < kMaxCluster && (heads * size < 2 * 148 || slots / size > kMaxKeys) && slots / size > 2048) size *= 2;
+  while (size < kMaxCluster && slots / size > 2048 && (heads * size * 2 <= 2 * 148 || slots / size > kMaxKeys)) size *= 2;
   return size;
 }
 
 template <bool KEEP_KEYS>
 cudaError_t launch(const EvictParams& p, int cluster, int smem, cudaStream_t st) {
-  auto kern = evict_kernel<KEEP_KEYS>;
+  auto kern = select_kernel<KEEP_KEYS>;
   cudaError_t e = allow_smem<std::integral_constant<bool, KEEP_KEYS>>(kern, kMaxKeys * 4);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
@@ -322,8 +349,18 @@ cudaError_t launch(const EvictParams& p, int cluster, int smem, cudaStream_t st)
 
 }  // namespace
 
+// The moves that one (sequence, KV head) can have: a free slot below keep, a slot from keep on.
+static int64_t most_moves(const SwaPagedEvictArgs& a) {
+  const int64_t behind = (int64_t)a.cache.max_pages * a.cache.page_size - a.keep;
+  return behind < 0 ? 0 : behind < a.keep ? behind : a.keep;
+}
+static size_t count_ints(const SwaPagedEvictArgs& a) {
+  return ((size_t)a.cache.batch * a.cache.n_kv_heads + 63) & ~(size_t)63;
+}
+
 size_t paged_evict_workspace(const SwaPagedEvictArgs& a) {
-  return ((size_t)a.cache.batch * a.cache.n_kv_heads * 2 * a.keep * sizeof(int32_t) + 255) & ~(size_t)255;
+  const size_t lists = (size_t)a.cache.batch * a.cache.n_kv_heads * 2 * most_moves(a);
+  return ((count_ints(a) + lists) * sizeof(int32_t) + 255) & ~(size_t)255;
 }
 
 cudaError_t launch_paged_evict(const PagedParams& c, const SwaPagedEvictArgs& a, cudaStream_t st) {
@@ -332,13 +369,17 @@ cudaError_t launch_paged_evict(const PagedParams& c, const SwaPagedEvictArgs& a,
   p.keep = a.keep; p.trigger = a.trigger; p.sink = a.sink_size; p.recent = a.recent;
   p.pieces = a.cache.head_dim / 8;
   p.piece_bits = p.pieces == 2 ? 1 : p.pieces == 4 ? 2 : p.pieces == 8 ? 3 : 4;
-  p.lists = static_cast<int32_t*>(a.workspace);
+  p.counts = static_cast<int32_t*>(a.workspace);
+  p.lists = p.counts + count_ints(a);
+  p.most = (int)most_moves(a);
   const int cluster = cluster_size(c);
   const int64_t slots = (int64_t)c.max_pages * c.page_size;
   const int64_t per = (slots + cluster * kThreads - 1) / (cluster * kThreads) * kThreads;
   cudaError_t e = per <= kMaxKeys ? launch<true>(p, cluster, (int)per * 4, st) : launch<false>(p, cluster, 0, st);
   if (e != cudaSuccess) return e;
-  return launch_pdl(evict_lens_kernel, (c.batch + 127) / 128, 128, 0, st, c, p.keep, p.trigger);
+  const int64_t x = ((int64_t)p.most * p.pieces + kMoveThreads * kMoves - 1) / (kMoveThreads * kMoves);
+  const int heads = c.batch * c.n_kv_heads;
+  return launch_pdl(move_kernel, dim3((unsigned)x, (unsigned)(heads < 65535 ? heads : 65535)), kMoveThreads, 0, st, p);
 }
 
 }  // namespace swa
