@@ -33,7 +33,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kUnit = 16;     // slots per unit
 constexpr int kSms = 148;
-constexpr int kWeightSlots = 512;  // slots per block of finish_kernel
+constexpr int kWeightSlots = 1024;  // slots per block of finish_kernel
 
 template <int D> struct Shape {
   static constexpr int kUnitBytes = 2 * kUnit * D * 2;  // K and V
@@ -426,7 +426,7 @@ struct Piece {
 };
 
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kernel(DecodeParams p) {
+__global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Piece pieces[kWarps][2];
   using P = Partial<D, ROWS>;
@@ -571,59 +571,63 @@ __device__ __forceinline__ void span_stats(const Span<D, ROWS>& s, int r, int la
   *l = ll;
 }
 
-// After decode_kernel.  Blocks [0, joins): one per (sequence, KV head, tile, row), which joins the
-// row's partials where the sequence spans blocks, each warp every fourth one.  Behind them, with
-// weights_out, blocks of kWeightSlots slots of a (sequence, KV head):
+// After decode_kernel.  Blocks [0, joins) join the rows of sequences that span blocks, `share` warps a
+// row.  Behind them, with weights_out, blocks of kWeightSlots slots of a (sequence, KV head):
 //   weights_out = decay * weights + sum over the heads of exp2(stored score - log-sum-exp),
 // with the log-sum-exp joined once more where it spans blocks, so that nothing waits for the joins.
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kThreads) finish_kernel(DecodeParams p, int grid, int joins, int weight_tiles) {
+__global__ void __launch_bounds__(kThreads, 8)
+finish_kernel(const __grid_constant__ DecodeParams p, int grid, int joins, int share, int weight_tiles) {
   using P = Partial<D, ROWS>;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, vh = p.c.n_kv_heads * p.tiles;
   if ((int)blockIdx.x < joins) {
     constexpr int V = D >= 32 ? D / 32 : 1;  // values of a lane
     __shared__ float sums[kWarps][D];
-    const int r = blockIdx.x % ROWS, bh = blockIdx.x / ROWS, b = bh / vh, hv = bh % vh;
-    const int row = hv % p.tiles * ROWS + r, head = hv / p.tiles * p.G + row;
-    if (row >= p.G) {
-      sm100::pdl_wait();  // (every block waits: the grid is not over before the one that it follows)
-      return;
-    }
-    const Span<D, ROWS> s(p, b, hv, grid);
-    const float sink = p.sinks ? p.sinks[head] * kLog2e : -INFINITY;
+    const int64_t at = (int64_t)blockIdx.x * (kWarps / share) + warp / share;
+    const int part = warp % share, r = (int)(at % ROWS);
+    const int64_t bh = at / ROWS;
+    const int b = (int)(bh / vh), hv = (int)(bh % vh), row = hv % p.tiles * ROWS + r, head = hv / p.tiles * p.G + row;
+    bool go = b < p.c.batch && row < p.G;
+    const Span<D, ROWS> s(p, go ? b : 0, go ? hv : 0, grid);
+    go = go && s.split();
+    const float sink = go && p.sinks ? p.sinks[head] * kLog2e : -INFINITY;
     sm100::pdl_wait();
-    if (!s.split()) return;
-    float m, l, acc[V] = {};
-    span_stats(s, r, lane, &m, &l);
-    const float base = m == -INFINITY ? 0.f : m;
+    float m = -INFINITY, l = 0.f, acc[V] = {};
     const bool live = lane * V < D;
+    if (go) {
+      span_stats(s, r, lane, &m, &l);
+      const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll 8
-    for (int c = s.c0 + warp; c <= s.c1; c += kWarps) {
-      float* q = s.part(c);
-      const float f = fast_exp2(P::m(q)[r] - base);
+      for (int c = s.c0 + part; c <= s.c1; c += share) {
+        float* q = s.part(c);
+        const float f = fast_exp2(P::m(q)[r] - base);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (live) acc[i] = fmaf(P::o(q)[r * D + lane * V + i], f, acc[i]);
+      }
+    }
+    if (share > 1) {
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        if (live) acc[i] = fmaf(P::o(q)[r * D + lane * V + i], f, acc[i]);
+        if (live) sums[warp][lane * V + i] = acc[i];
+      __syncthreads();
     }
+    if (!go || part) return;
+    const Row w = finish(m, l, sink);
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (live) sums[warp][lane * V + i] = acc[i];
-    __syncthreads();
-    const Row w = finish(m, l, sink);
-    for (int d = threadIdx.x; d < D; d += kThreads) {
-      float x = 0.f;
-#pragma unroll
-      for (int i = 0; i < kWarps; ++i) x += sums[i][d];
-      static_cast<T*>(p.o)[b * p.ob + head * p.oh + d] = Pack<T>::from(x * w.inv);
-    }
-    if (p.lse && threadIdx.x == 0) p.lse[(int64_t)b * p.Hq + head] = w.lse;
+      if (live) {
+        for (int j = 1; j < share; ++j) acc[i] += sums[warp + j][lane * V + i];
+        static_cast<T*>(p.o)[b * p.ob + head * p.oh + lane * V + i] = Pack<T>::from(acc[i] * w.inv);
+      }
+    if (p.lse && lane == 0) p.lse[(int64_t)b * p.Hq + head] = w.lse;
     return;
   }
   const int at = blockIdx.x - joins, hk = at / weight_tiles % p.c.n_kv_heads, b = at / weight_tiles / p.c.n_kv_heads;
   const Sequence s = sequence(p, b);
   const int slot0 = at % weight_tiles * kWeightSlots;
   if (slot0 >= s.n) {
-    sm100::pdl_wait();
+    sm100::pdl_wait();  // (every block waits: the grid is not over before the one that it follows)
     return;
   }
   constexpr int kPer = kWeightSlots / kThreads;
@@ -634,21 +638,22 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(DecodeParams p, int gr
     const int slot = slot0 + i * kThreads + threadIdx.x;
     w[i] = slot < s.n && p.c.weights ? p.decay * p.c.weights[b * p.c.wb + hk * p.c.wh + slot] : 0.f;
   }
+  const Span<D, ROWS> all(p, b, hk * p.tiles, p.warps ? 1 : grid);
   sm100::pdl_wait();
   for (int tile = 0; tile < p.tiles; ++tile) {
     const int hv = hk * p.tiles + tile, rows = p.G - tile * ROWS < ROWS ? p.G - tile * ROWS : ROWS;
+    const float* finished = p.lse + (int64_t)b * p.Hq + hk * p.G + tile * ROWS;
     __syncthreads();
     if (p.warps) {
-      if ((int)threadIdx.x < rows) lse[threadIdx.x] = p.lse[(int64_t)b * p.Hq + hk * p.G + tile * ROWS + threadIdx.x];
+      if ((int)threadIdx.x < rows) lse[threadIdx.x] = finished[threadIdx.x];
     } else {
-      const Span<D, ROWS> span(p, b, hv, grid);
+      const Span<D, ROWS> span = tile ? Span<D, ROWS>(p, b, hv, grid) : all;
       for (int r = warp; r < rows; r += kWarps) {
-        const int head = hk * p.G + tile * ROWS + r;
         float m = 0.f, l = 0.f;
         if (span.split()) span_stats(span, r, lane, &m, &l);
         if (lane == 0)
-          lse[r] = span.split() ? finish(m, l, p.sinks ? p.sinks[head] * kLog2e : -INFINITY).lse
-                                : p.lse[(int64_t)b * p.Hq + head];
+          lse[r] = span.split() ? finish(m, l, p.sinks ? p.sinks[hk * p.G + tile * ROWS + r] * kLog2e : -INFINITY).lse
+                                : finished[r];
       }
     }
     __syncthreads();
@@ -731,12 +736,16 @@ cudaError_t launch(const DecodeParams& p, const Plan& pl, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   kern<<<pl.blocks, kThreads, smem, st>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  const int64_t joins = p.warps ? 0 : (int64_t)p.c.batch * p.c.n_kv_heads * p.tiles * ROWS;
+  // four warps a row where the rows alone do not fill the GPU and their spans are long
+  const int64_t rows = (int64_t)p.c.batch * p.c.n_kv_heads * p.tiles * ROWS;
+  const int share = rows <= kSms * 8 ? kWarps : 1;
+  const int64_t joins = p.warps ? 0 : (rows * share + kWarps - 1) / kWarps;
   const int64_t slots = (int64_t)p.c.max_pages * p.c.page_size;
   const int64_t tiles = p.wout ? (slots + kWeightSlots - 1) / kWeightSlots : 0;
   const int64_t blocks = joins + tiles * p.c.n_kv_heads * p.c.batch;
   if (blocks == 0) return cudaSuccess;
-  return launch_pdl(finish_kernel<T, D, ROWS>, (int)blocks, kThreads, 0, st, p, pl.blocks, (int)joins, (int)tiles);
+  return launch_pdl(finish_kernel<T, D, ROWS>, (unsigned)blocks, kThreads, 0, st, p, pl.blocks, (int)joins, share,
+                    (int)tiles);
 }
 
 template <typename T, int ROWS>
