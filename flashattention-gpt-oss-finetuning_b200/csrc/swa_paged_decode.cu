@@ -37,9 +37,11 @@ constexpr int kWeightSlots = 1024;  // slots per block of finish_kernel
 
 template <int D> struct Shape {
   static constexpr int kUnitBytes = 2 * kUnit * D * 2;  // K and V
-  static constexpr int kStages = D == 128 ? 3 : 4;
+  // Three stages and four blocks an SM (128 registers a thread): 97 us where four and three take 101
+  // (32 sequences of up to 16384 slots, D 64), and 256 windows fit in one wave (17 us, not 23).
+  static constexpr int kStages = 3;
   static constexpr int kRing = kStages * kUnitBytes;    // per warp
-  static constexpr int kBlocksPerSm = D == 128 ? 2 : 3;
+  static constexpr int kBlocksPerSm = D == 128 ? 2 : 4;
   static constexpr int kMaxBlocks = kSms * kBlocksPerSm;
 };
 
@@ -148,7 +150,11 @@ __device__ __forceinline__ void ldsm4t(uint32_t* r, uint32_t addr) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
 }
-// 16 bytes to shared memory, zeros where !ok (then nothing is read)
+// 16 bytes to shared memory
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// the same, zeros where !ok (then nothing is read)
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
@@ -197,41 +203,67 @@ template <typename T, int D, int ROWS> struct Walk {
 #pragma unroll
     for (int i = 0; i < kHalves; ++i) m[i] = -INFINITY, l[i] = 0.f;
 
-    const T* kbase = static_cast<const T*>(p.c.k) + h * p.c.kh;
-    const T* vbase = static_cast<const T*>(p.c.v) + h * p.c.vh;
+    // A lane copies kCopies pieces of K and of V of every unit, kRows rows apart.
+    constexpr int kPieces = D / 8, kCopies = kUnit * kPieces / 32, kRows = 32 / kPieces;
+    const int row0 = lane / kPieces, piece = lane % kPieces;
+    const T* kbase = static_cast<const T*>(p.c.k) + h * p.c.kh + row0 * p.c.kr + piece * 8;
+    const T* vbase = static_cast<const T*>(p.c.v) + h * p.c.vh + row0 * p.c.vr + piece * 8;
+    const int64_t kstep = kRows * p.c.kr, vstep = kRows * p.c.vr;
+    uint32_t to[kCopies];
+#pragma unroll
+    for (int e = 0; e < kCopies; ++e) to[e] = swizzled<D>(row0 + e * kRows, piece);
 
     // page of unit u0 + 32 i + lane, looked up 32 units at a time
+    const int upp = p.units_per_page;
     auto pages = [&](int u) -> int {
       if (u >= u1) return -1;
       const int chunk = unit_chunk(s, u);
       if (chunk * kUnit >= s.n) return -1;
-      return paged_page(p.c, b, chunk / p.units_per_page, &bad);
+      return paged_page(p.c, b, chunk / upp, &bad);
     };
     int ids = pages(u0 + lane);
-    const int upp = p.units_per_page;
+    // the loads' place: unit, its chunk, the chunk's place in its page, the ring's stage
+    int lu = u0, lchunk = unit_chunk(s, u0), lin = lchunk % upp, lstage = 0;
 
-    auto issue = [&](int u) {
-      if (u < u1) {
-        const int i = u - u0;
-        if (i && (i & 31) == 0) ids = pages(u + lane);
-        const int page = __shfl_sync(~0u, ids, i & 31);
-        const int chunk = unit_chunk(s, u), slot0 = chunk * kUnit, row0 = (chunk % upp) * kUnit;
-        const T* kp = kbase + (page < 0 ? 0 : page) * p.c.kp + (int64_t)row0 * p.c.kr;
-        const T* vp = vbase + (page < 0 ? 0 : page) * p.c.vp + (int64_t)row0 * p.c.vr;
-        const uint32_t dst = ring + (uint32_t)(i % kStages) * Shape<D>::kUnitBytes;
-        constexpr int kPieces = D / 8;
+    auto issue = [&]() {
+      if (lu < u1) {
+        const int i = (lu - u0) & 31;
+        if (i == 0 && lu != u0) ids = pages(lu + lane);
+        const int page = __shfl_sync(~0u, ids, i), slot0 = lchunk * kUnit;
+        const T* kp = kbase + (page < 0 ? 0 : page) * p.c.kp + lin * (kUnit * p.c.kr);
+        const T* vp = vbase + (page < 0 ? 0 : page) * p.c.vp + lin * (kUnit * p.c.vr);
+        const uint32_t kd = ring + (uint32_t)lstage * Shape<D>::kUnitBytes, vd = kd + kUnit * D * 2;
+        if (page >= 0 && slot0 + kUnit <= s.n && (slot0 >= s.first || slot0 + kUnit <= s.sinks)) {
 #pragma unroll
-        for (int e = 0; e < kUnit * kPieces; e += 32) {
-          const int at = e + lane, row = at / kPieces, piece = at % kPieces, slot = slot0 + row;
-          const bool ok = page >= 0 && slot < s.n && (slot >= s.first || slot < s.sinks);
-          copy16(dst + swizzled<D>(row, piece), kp + row * p.c.kr + piece * 8, ok);
-          copy16(dst + kUnit * D * 2 + swizzled<D>(row, piece), vp + row * p.c.vr + piece * 8, ok);
+          for (int e = 0; e < kCopies; ++e) {
+            copy16(kd + to[e], kp);
+            copy16(vd + to[e], vp);
+            kp += kstep;
+            vp += vstep;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < kCopies; ++e) {
+            const int slot = slot0 + row0 + e * kRows;
+            const bool ok = page >= 0 && slot < s.n && (slot >= s.first || slot < s.sinks);
+            copy16(kd + to[e], kp, ok);
+            copy16(vd + to[e], vp, ok);
+            kp += kstep;
+            vp += vstep;
+          }
         }
+        ++lchunk;
+        if (++lin == upp) lin = 0;
+        if (++lu == s.a) {
+          lchunk = s.c0;
+          lin = lchunk % upp;
+        }
+        if (++lstage == kStages) lstage = 0;
       }
       copy_commit();
     };
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) issue(u0 + i);
+    for (int i = 0; i < kStages - 1; ++i) issue();
 
     // Q as the A operand, rows past the group's heads as zeros
     uint32_t qa[kKs][4];
@@ -247,30 +279,41 @@ template <typename T, int D, int ROWS> struct Walk {
                         : 0u;
       }
 
+    // Addresses of the matrices in a unit: pieces differ in address bits that the swizzle's are
+    // exclusive-ored into, so a piece further on is an exclusive or away.
+    const uint32_t kfrag = ring + swizzled<D>((lane >> 4) * 8 + (lane & 7), (lane >> 3) & 1);
+    const uint32_t vfrag = ring + kUnit * D * 2 + swizzled<D>(((lane >> 3) & 1) * 8 + (lane & 7), lane >> 4);
+    int chunk = unit_chunk(s, u0);
+    uint32_t stage = 0;
     for (int u = u0; u < u1; ++u) {
-      issue(u + kStages - 1);
+      issue();
       copy_wait<kStages - 1>();
       __syncwarp();
-      const uint32_t kt = ring + (uint32_t)((u - u0) % kStages) * Shape<D>::kUnitBytes, vt = kt + kUnit * D * 2;
       float sc[2][4] = {};
 #pragma unroll
       for (int ks = 0; ks < kKs; ++ks) {
         uint32_t kb[4];
-        ldsm4(kb, kt + swizzled<D>((lane >> 4) * 8 + (lane & 7), ks * 2 + ((lane >> 3) & 1)));
+        ldsm4(kb, (kfrag + stage) ^ (ks * 32));
         mma16816<T>(sc[0], qa[ks], kb[0], kb[1]);
         mma16816<T>(sc[1], qa[ks], kb[2], kb[3]);
       }
-      const int slot0 = unit_chunk(s, u) * kUnit;
+      const int slot0 = chunk * kUnit;
       const bool full = slot0 + kUnit <= s.n && (slot0 >= s.first || slot0 + kUnit <= s.sinks);
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int slot = slot0 + 8 * j + 2 * t + e;
-          const bool ok = full || (slot < s.n && (slot >= s.first || slot < s.sinks));
+        for (int e = 0; e < 2 * kHalves; ++e) sc[j][e] *= p.scale_log2;
+      if (!full) {
 #pragma unroll
-          for (int r = 0; r < kHalves; ++r) sc[j][2 * r + e] = ok ? sc[j][2 * r + e] * p.scale_log2 : -INFINITY;
-        }
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int slot = slot0 + 8 * j + 2 * t + e;
+            if (slot >= s.n || (slot < s.first && slot >= s.sinks))
+#pragma unroll
+              for (int r = 0; r < kHalves; ++r) sc[j][2 * r + e] = -INFINITY;
+          }
+      }
       if (p.scores) {
         float* out = p.scores + (((int64_t)b * p.c.n_kv_heads * p.tiles + hv) * p.max_units + u) * (ROWS * kUnit);
 #pragma unroll
@@ -278,7 +321,8 @@ template <typename T, int D, int ROWS> struct Walk {
 #pragma unroll
           for (int r = 0; r < kHalves; ++r)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) out[(8 * j + 2 * t + e) * ROWS + g + 8 * r] = sc[j][2 * r + e];
+            for (int e = 0; e < 2; ++e)
+              out[(8 * j + 2 * t + e) * ROWS + g + 8 * r] = tile * ROWS + g + 8 * r < p.G ? sc[j][2 * r + e] : -INFINITY;
       }
       float up[kHalves];
       bool grew = false;
@@ -321,7 +365,7 @@ template <typename T, int D, int ROWS> struct Walk {
 #pragma unroll
       for (int i = 0; i < kNt; i += 2) {
         uint32_t vb[4];
-        ldsm4t(vb, vt + swizzled<D>(((lane >> 3) & 1) * 8 + (lane & 7), i + (lane >> 4)));
+        ldsm4t(vb, (vfrag + stage) ^ (i * 16));
         if (kHalves == 1) {
           const uint32_t a[4] = {hi[0][0], lo[0][0], hi[0][1], lo[0][1]};
           mma16816<T>(o[i], a, vb[0], vb[1]);
@@ -336,6 +380,9 @@ template <typename T, int D, int ROWS> struct Walk {
         }
       }
       __syncwarp();
+      chunk = u + 1 == s.a ? s.c0 : chunk + 1;
+      stage += Shape<D>::kUnitBytes;
+      if (stage == Shape<D>::kRing) stage = 0;
     }
     copy_wait<0>();
     __syncwarp();
@@ -427,7 +474,7 @@ struct Piece {
 
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kernel(const __grid_constant__ DecodeParams p) {
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ Piece pieces[kWarps][2];
   using P = Partial<D, ROWS>;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -631,49 +678,49 @@ finish_kernel(const __grid_constant__ DecodeParams p, int grid, int joins, int s
     return;
   }
   constexpr int kPer = kWeightSlots / kThreads;
-  __shared__ float lse[ROWS];
+  __shared__ float shared_lse[ROWS];
   float w[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int slot = slot0 + i * kThreads + threadIdx.x;
     w[i] = slot < s.n && p.c.weights ? p.decay * p.c.weights[b * p.c.wb + hk * p.c.wh + slot] : 0.f;
   }
-  const Span<D, ROWS> all(p, b, hk * p.tiles, p.warps ? 1 : grid);
+  Span<D, ROWS> span(p, b, hk * p.tiles, p.warps ? 1 : grid);
+  const int gap = (s.c0 - s.a) * kUnit;  // slots between the sinks' units and the window's
   sm100::pdl_wait();
   for (int tile = 0; tile < p.tiles; ++tile) {
-    const int hv = hk * p.tiles + tile, rows = p.G - tile * ROWS < ROWS ? p.G - tile * ROWS : ROWS;
-    const float* finished = p.lse + (int64_t)b * p.Hq + hk * p.G + tile * ROWS;
-    __syncthreads();
-    if (p.warps) {
-      if ((int)threadIdx.x < rows) lse[threadIdx.x] = finished[threadIdx.x];
+    const int rows = p.G - tile * ROWS < ROWS ? p.G - tile * ROWS : ROWS, head0 = hk * p.G + tile * ROWS;
+    const float* finished = p.lse + (int64_t)b * p.Hq + head0;
+    if (tile) {
+      __syncthreads();
+      if (!p.warps) span = Span<D, ROWS>(p, b, hk * p.tiles + tile, grid);
+    }
+    if (p.warps || !span.split()) {
+      if ((int)threadIdx.x < ROWS) shared_lse[threadIdx.x] = (int)threadIdx.x < rows ? finished[threadIdx.x] : 0.f;
     } else {
-      const Span<D, ROWS> span = tile ? Span<D, ROWS>(p, b, hv, grid) : all;
-      for (int r = warp; r < rows; r += kWarps) {
-        float m = 0.f, l = 0.f;
-        if (span.split()) span_stats(span, r, lane, &m, &l);
+      for (int r = warp; r < ROWS; r += kWarps) {
+        float m = -INFINITY, l = 0.f;
+        if (r < rows) span_stats(span, r, lane, &m, &l);
         if (lane == 0)
-          lse[r] = span.split() ? finish(m, l, p.sinks ? p.sinks[hk * p.G + tile * ROWS + r] * kLog2e : -INFINITY).lse
-                                : finished[r];
+          shared_lse[r] = r < rows ? finish(m, l, p.sinks ? p.sinks[head0 + r] * kLog2e : -INFINITY).lse : 0.f;
       }
     }
     __syncthreads();
+    float lse[ROWS];  // rows without a head add 0: their scores are -inf
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) lse[r] = shared_lse[r];
+    const float* scores = p.scores + (((int64_t)b * vh + hk * p.tiles + tile) * p.max_units) * (ROWS * kUnit);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int slot = slot0 + i * kThreads + threadIdx.x;
       if (slot < s.n && (slot < s.sinks || slot >= s.first)) {
-        const int chunk = slot / kUnit, u = chunk < s.a ? chunk : chunk - s.c0 + s.a;
-        const float4* sc = reinterpret_cast<const float4*>(
-            p.scores + (((int64_t)b * vh + hv) * p.max_units + u) * (ROWS * kUnit) + slot % kUnit * ROWS);
+        const float4* sc = reinterpret_cast<const float4*>(scores + (int64_t)(slot < s.a * kUnit ? slot : slot - gap) * ROWS);
         float sum = 0.f;
 #pragma unroll
         for (int r = 0; r < ROWS; r += 4) {
-          if (r < rows) {
-            const float4 x = sc[r / 4];
-            sum += fast_exp2(x.x - lse[r]);
-            if (r + 1 < rows) sum += fast_exp2(x.y - lse[r + 1]);
-            if (r + 2 < rows) sum += fast_exp2(x.z - lse[r + 2]);
-            if (r + 3 < rows) sum += fast_exp2(x.w - lse[r + 3]);
-          }
+          const float4 x = sc[r / 4];
+          sum += (fast_exp2(x.x - lse[r]) + fast_exp2(x.y - lse[r + 1])) +
+                 (fast_exp2(x.z - lse[r + 2]) + fast_exp2(x.w - lse[r + 3]));
         }
         w[i] += sum;
       }
