@@ -432,36 +432,42 @@ template <typename T, int D, int ROWS> struct Walk {
   }
 };
 
-// Joins `count` partials at part(0 ..) of one (sequence, KV head, tile) by all threads of the block:
-// into the output, or into `into` where it is given.
-template <typename T, int D, int ROWS, typename F>
-__device__ __forceinline__ void join(const DecodeParams& p, int b, int hv, int count, F part, float* into) {
+// Joins up to kMost partials, at part[0 .. count), of one (sequence, KV head, tile) by all threads of
+// the block: into the output, or into `into` where it is given.
+template <typename T, int D, int ROWS, int kMost>
+__device__ __forceinline__ void join(const DecodeParams& p, int b, int hv, int count, float* const (&part)[kMost],
+                                     float* into) {
   using P = Partial<D, ROWS>;
   const int h = hv / p.tiles, tile = hv % p.tiles;
   const int rows = p.G - tile * ROWS < ROWS ? p.G - tile * ROWS : ROWS;
   for (int e = threadIdx.x; e < rows * (D / 2); e += kThreads) {
     const int r = e / (D / 2), d = e % (D / 2) * 2;
-    float m = -INFINITY;
-    for (int i = 0; i < count; ++i) m = fmaxf(m, P::m(part(i))[r]);
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f, x = 0.f, y = 0.f;
-    for (int i = 0; i < count; ++i) {
-      float* q = part(i);
-      const float f = fast_exp2(P::m(q)[r] - base);
-      const float2 v = *reinterpret_cast<const float2*>(P::o(q) + r * D + d);
-      l = fmaf(P::l(q)[r], f, l);
-      x = fmaf(v.x, f, x);
-      y = fmaf(v.y, f, y);
+    float m[kMost], top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+      m[i] = i < count ? P::m(part[i])[r] : -INFINITY;
+      top = fmaxf(top, m[i]);
     }
+    const float base = top == -INFINITY ? 0.f : top;
+    float l = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i)
+      if (i < count) {
+        const float f = fast_exp2(m[i] - base);
+        const float2 v = *reinterpret_cast<const float2*>(P::o(part[i]) + r * D + d);
+        l = fmaf(P::l(part[i])[r], f, l);
+        x = fmaf(v.x, f, x);
+        y = fmaf(v.y, f, y);
+      }
     if (into) {
       if (d == 0) {
-        P::m(into)[r] = m;
+        P::m(into)[r] = top;
         P::l(into)[r] = l;
       }
       *reinterpret_cast<float2*>(P::o(into) + r * D + d) = make_float2(x, y);
     } else {
       const int head = h * p.G + tile * ROWS + r;
-      const Row w = finish(m, l, p.sinks ? p.sinks[head] * kLog2e : -INFINITY);
+      const Row w = finish(top, l, p.sinks ? p.sinks[head] * kLog2e : -INFINITY);
       *reinterpret_cast<uint32_t*>(static_cast<T*>(p.o) + b * p.ob + head * p.oh + d) = Pack<T>::pack(x * w.inv, y * w.inv);
       if (p.lse && d == 0) p.lse[(int64_t)b * p.Hq + head] = w.lse;
     }
@@ -492,9 +498,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kerne
     b = (int)(at / vh);
     hv = (int)(at % vh);
     s = sequence(p, b);
-    const int part = warp % p.warps;
-    u = s.units * part / p.warps;
-    todo = s.units * (part + 1) / p.warps - u;
+    const int part = warp % p.warps, share = (s.units + p.warps - 1) / p.warps;
+    u = min(part * share, s.units);
+    todo = min(u + share, s.units) - u;
   } else {
     int per;
     const int64_t mine = lane_units(p, lane, &per);
@@ -542,6 +548,17 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kerne
   if (p.warps == 1) return;
   __syncthreads();
 
+  if (p.warps) {  // one (sequence, KV head, tile), its pieces in the first warps' rings
+    float* part[kWarps];
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      part[i] = reinterpret_cast<float*>(smem + i * Shape<D>::kRing);
+      count += pieces[i][1].bh >= 0;
+    }
+    if (count) join<T, D, ROWS>(p, b, hv, count, part, nullptr);  // (none: a warp walked it whole)
+    return;
+  }
   // join neighbouring pieces of the same (sequence, KV head, tile)
   for (int i = 0; i < 2 * kWarps;) {
     const Piece a = pieces[i / 2][i % 2];
@@ -549,22 +566,25 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kerne
       ++i;
       continue;
     }
-    int at[2 * kWarps], count = 0, end = a.u1;
-    at[count++] = i++;
-    for (; i < 2 * kWarps; ++i) {
-      const Piece& c = pieces[i / 2][i % 2];
-      if (c.bh < 0) continue;
-      if (c.bh != a.bh) break;
-      at[count++] = i;
-      end = c.u1;
+    float* part[kWarps];  // at most one of every warp
+    int count = 0, end = a.u1;
+#pragma unroll
+    for (int j = 0; j < 2 * kWarps; ++j) {
+      if (j < i || pieces[j / 2][j % 2].bh != a.bh) continue;
+      float* at = j % 2 ? reinterpret_cast<float*>(smem + j / 2 * Shape<D>::kRing)
+                        : p.heads + ((int64_t)blockIdx.x * kWarps + j / 2) * P::kFloats;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k)  // (a place known at compile time: registers)
+        if (k == count) part[k] = at;
+      ++count;
+      end = pieces[j / 2][j % 2].u1;
     }
+    int last = i;  // a sequence's pieces are neighbours, but for warps without that piece
+    for (int j = i; j < 2 * kWarps; ++j)
+      if (pieces[j / 2][j % 2].bh == a.bh) last = j;
+    i = last + 1;
     const bool done = a.u0 == 0 && end == a.units;
     float* into = done ? nullptr : p.partials + ((int64_t)blockIdx.x * 2 + (a.u0 > 0 ? 0 : 1)) * P::kFloats;
-    auto part = [&](int k) -> float* {
-      const int x = at[k];
-      return x % 2 ? reinterpret_cast<float*>(smem + x / 2 * Shape<D>::kRing)
-                   : p.heads + ((int64_t)blockIdx.x * kWarps + x / 2) * P::kFloats;
-    };
     join<T, D, ROWS>(p, a.bh / vh, a.bh % vh, count, part, into);
   }
 }
@@ -740,9 +760,14 @@ struct Plan {
 };
 size_t round64(size_t n) { return (n + 63) & ~(size_t)63; }
 
-// Visible units from which sequences are dealt out over blocks: below, a block of its own is as
-// quick and saves the join.
-constexpr int kWholeUnits = 32;
+#ifndef V_U1
+#define V_U1 32
+#define V_U4 136
+#define V_SEQ 96
+#endif
+// Visible units up to which a (sequence, KV head) is one warp's or one block's, so that nothing is
+// left to join, where there are enough of them to fill the GPU.
+constexpr int kUnitsWarp = V_U1, kUnitsBlock = V_U4, kSeqsBlock = V_SEQ;
 
 Plan plan(const SwaPagedDecodeArgs& a) {
   const SwaPagedKV& c = a.cache;
@@ -759,9 +784,9 @@ Plan plan(const SwaPagedDecodeArgs& a) {
   r.max_units = units > 0 ? (int)units : 1;
   const int64_t seqs = (int64_t)c.batch * c.n_kv_heads * r.tiles;
   const int most = D == 128 ? Shape<128>::kMaxBlocks : Shape<64>::kMaxBlocks;
-  if (r.max_units <= kWholeUnits) {
-    // a warp each where that fills the GPU: no join, and four times as many in flight
-    r.warps = seqs >= most ? 1 : kWarps;
+  if (r.max_units <= kUnitsWarp) r.warps = seqs >= most ? 1 : kWarps;
+  else if (r.max_units <= kUnitsBlock && seqs >= kSeqsBlock) r.warps = kWarps;
+  if (r.warps) {
     r.blocks = (int)((seqs * r.warps + kWarps - 1) / kWarps);
   } else {
     const int64_t want = (seqs * r.max_units + 2 * kWarps - 1) / (2 * kWarps);
