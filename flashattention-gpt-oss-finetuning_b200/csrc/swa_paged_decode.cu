@@ -61,6 +61,7 @@ struct DecodeParams {
   float decay;
   float* partials;         // [blocks][2] Partial
   float* heads;            // [blocks][warps] Partial: the first piece of a warp that has two
+  int2* spans;             // [B * Hkv * tiles]: first and last block, where dealt out
   float* scores;           // [B * Hkv * tiles][max_units][16][ROWS]
 };
 
@@ -478,10 +479,17 @@ struct Piece {
   int bh, u0, u1, units;
 };
 
+// A warp's place among all units, in shared memory: it is wanted between sequences alone.
+struct Deal {
+  int64_t at, total;
+  int blocks;
+};
+
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ Piece pieces[kWarps][2];
+  __shared__ Deal deals[kWarps];
   using P = Partial<D, ROWS>;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int vh = p.c.n_kv_heads * p.tiles;
@@ -493,10 +501,10 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kerne
   int64_t todo;
   Sequence s;
   if (p.warps) {
-    const int64_t at = (int64_t)blockIdx.x * (kWarps / p.warps) + warp / p.warps;
-    if (at >= (int64_t)p.c.batch * vh) return;  // (warps of the last block, where p.warps is 1)
-    b = (int)(at / vh);
-    hv = (int)(at % vh);
+    const int bh = blockIdx.x * (kWarps / p.warps) + warp / p.warps;
+    if (bh >= p.c.batch * vh) return;  // (warps of the last block, where p.warps is 1)
+    b = bh / vh;
+    hv = bh % vh;
     s = sequence(p, b);
     const int part = warp % p.warps, share = (s.units + p.warps - 1) / p.warps;
     u = min(part * share, s.units);
@@ -508,12 +516,12 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kerne
     const int blocks = active_blocks(total, gridDim.x);
     if ((int)blockIdx.x >= blocks) return;
     const int64_t b0 = total * blockIdx.x / blocks, b1 = total * (blockIdx.x + 1) / blocks;
-    const int64_t start = b0 + (b1 - b0) * warp / kWarps;
-    todo = b0 + (b1 - b0) * (warp + 1) / kWarps - start;
-    // the lane whose sequences hold `start`, then the sequence
-    const unsigned has = __ballot_sync(~0u, start >= before && start < before + mine * vh);
+    const int64_t at = b0 + (b1 - b0) * warp / kWarps;
+    todo = b0 + (b1 - b0) * (warp + 1) / kWarps - at;
+    // the lane whose sequences hold `at`, then the sequence
+    const unsigned has = __ballot_sync(~0u, at >= before && at < before + mine * vh);
     const int src = has ? __ffs(has) - 1 : 0;
-    int64_t rest = start - __shfl_sync(~0u, before, src);
+    int64_t rest = at - __shfl_sync(~0u, before, src);
     b = src * per;
     s = sequence(p, b);
     while (todo > 0 && rest >= (int64_t)s.units * vh) {
@@ -522,12 +530,19 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kerne
     }
     hv = (int)(rest / s.units);
     u = (int)(rest % s.units);
+    if (lane == 0) deals[warp] = {at, total, blocks};
   }
   if (lane < 2) pieces[warp][lane].bh = -1;
   __syncwarp();
   Walk<T, D, ROWS> w;
   while (todo > 0) {
     const int u1 = (int)(todo < s.units - u ? u + todo : s.units);
+    if (!p.warps && lane == 0) {
+      Deal& d = deals[warp];
+      // block c holds units [total c / blocks, total (c + 1) / blocks)
+      if (u == 0) p.spans[b * vh + hv] = make_int2(blockIdx.x, (int)(((d.at + s.units) * d.blocks - 1) / d.total));
+      d.at += u1 - u;
+    }
     w.run(p, saddr(ring), lane, b, hv, s, u, u1);
     todo -= u1 - u;
     if (u == 0 && u1 == s.units) {
@@ -589,32 +604,17 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kerne
   }
 }
 
-// The blocks of decode_kernel that hold units of (b, hv), found by the same dealing out, and their
-// partials.
+// The blocks that hold units of one (sequence, KV head, tile), and their partials.
 template <int D, int ROWS> struct Span {
-  int c0, c1, blocks;
-  int64_t total, start;
+  int c0, c1;
   float* partials;
-  __device__ __forceinline__ Span(const DecodeParams& p, int b, int hv, int grid) {
-    const int lane = threadIdx.x % 32, vh = p.c.n_kv_heads * p.tiles;
-    int64_t all = 0, before = 0;
-    int units = 0;
-    for (int i = lane; i < p.c.batch; i += 32) {
-      const int n = sequence(p, i).units;
-      all += n;
-      if (i < b) before += n;
-      if (i == b) units = n;
-    }
-    units = __shfl_sync(~0u, units, b % 32);
-    total = warp_sum(all) * vh;
-    start = warp_sum(before) * vh + (int64_t)hv * units;
-    blocks = active_blocks(total, grid);
-    // block c holds [total c / blocks, total (c + 1) / blocks)
-    c0 = (int)(((start + 1) * blocks - 1) / total);
-    c1 = (int)(((start + units) * blocks - 1) / total);
-    partials = p.partials;
+  __device__ __forceinline__ Span(const DecodeParams& p, int bh) : partials(p.partials) {
+    const int2 s = p.warps ? make_int2(0, 0) : p.spans[bh];
+    c0 = s.x;
+    c1 = s.y;
   }
   __device__ __forceinline__ bool split() const { return c1 > c0; }
+  // The first block's last run of units, the others' first.
   __device__ __forceinline__ float* part(int c) const {
     return partials + ((int64_t)c * 2 + (c > c0 ? 0 : 1)) * Partial<D, ROWS>::kFloats;
   }
@@ -638,55 +638,72 @@ __device__ __forceinline__ void span_stats(const Span<D, ROWS>& s, int r, int la
   *l = ll;
 }
 
+// Adds partial (mi, li, oi) of a row to (m, l, acc).
+template <int V>
+__device__ __forceinline__ void join_row(float* m, float* l, float* acc, float mi, float li, const float* oi) {
+  const float up = fmaxf(*m, mi), base = up == -INFINITY ? 0.f : up;
+  const float f = fast_exp2(*m - base), g = fast_exp2(mi - base);
+  *m = up;
+  *l = *l * f + li * g;
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] = acc[i] * f + oi[i] * g;
+}
+
 // After decode_kernel.  Blocks [0, joins) join the rows of sequences that span blocks, `share` warps a
 // row.  Behind them, with weights_out, blocks of kWeightSlots slots of a (sequence, KV head):
 //   weights_out = decay * weights + sum over the heads of exp2(stored score - log-sum-exp),
 // with the log-sum-exp joined once more where it spans blocks, so that nothing waits for the joins.
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(kThreads, 8)
-finish_kernel(const __grid_constant__ DecodeParams p, int grid, int joins, int share, int weight_tiles) {
+finish_kernel(const __grid_constant__ DecodeParams p, int joins, int share, int weight_tiles) {
   using P = Partial<D, ROWS>;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, vh = p.c.n_kv_heads * p.tiles;
   if ((int)blockIdx.x < joins) {
     constexpr int V = D >= 32 ? D / 32 : 1;  // values of a lane
-    __shared__ float sums[kWarps][D];
-    const int64_t at = (int64_t)blockIdx.x * (kWarps / share) + warp / share;
-    const int part = warp % share, r = (int)(at % ROWS);
-    const int64_t bh = at / ROWS;
-    const int b = (int)(bh / vh), hv = (int)(bh % vh), row = hv % p.tiles * ROWS + r, head = hv / p.tiles * p.G + row;
+    __shared__ float sums[kWarps][D], stats[kWarps][2];
+    const int at = blockIdx.x * (kWarps / share) + warp / share, bh = at / ROWS, r = at % ROWS, sub = warp % share;
+    const int b = bh / vh, hv = bh % vh, row = hv % p.tiles * ROWS + r, head = hv / p.tiles * p.G + row;
     bool go = b < p.c.batch && row < p.G;
-    const Span<D, ROWS> s(p, go ? b : 0, go ? hv : 0, grid);
-    go = go && s.split();
     const float sink = go && p.sinks ? p.sinks[head] * kLog2e : -INFINITY;
     sm100::pdl_wait();
+    const Span<D, ROWS> s(p, go ? bh : 0);
+    go = go && s.split();
     float m = -INFINITY, l = 0.f, acc[V] = {};
     const bool live = lane * V < D;
-    if (go) {
-      span_stats(s, r, lane, &m, &l);
-      const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll 8
-      for (int c = s.c0 + part; c <= s.c1; c += share) {
-        float* q = s.part(c);
-        const float f = fast_exp2(P::m(q)[r] - base);
+    constexpr int kAhead = 4;
+    if (go)
+      for (int c = s.c0 + sub; c <= s.c1; c += share * kAhead) {
+        float mi[kAhead], li[kAhead], oi[kAhead][V];
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (live) acc[i] = fmaf(P::o(q)[r * D + lane * V + i], f, acc[i]);
+        for (int j = 0; j < kAhead; ++j) {
+          const bool in = c + j * share <= s.c1;
+          float* q = s.part(in ? c + j * share : c);
+          mi[j] = in ? P::m(q)[r] : -INFINITY;
+          li[j] = in ? P::l(q)[r] : 0.f;
+#pragma unroll
+          for (int i = 0; i < V; ++i) oi[j][i] = in && live ? P::o(q)[r * D + lane * V + i] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) join_row<V>(&m, &l, acc, mi[j], li[j], oi[j]);
       }
-    }
     if (share > 1) {
 #pragma unroll
       for (int i = 0; i < V; ++i)
         if (live) sums[warp][lane * V + i] = acc[i];
+      if (lane == 0) stats[warp][0] = m, stats[warp][1] = l;
       __syncthreads();
     }
-    if (!go || part) return;
+    if (!go || sub) return;
+    for (int j = 1; j < share; ++j) {
+      float other[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) other[i] = live ? sums[warp + j][lane * V + i] : 0.f;
+      join_row<V>(&m, &l, acc, stats[warp + j][0], stats[warp + j][1], other);
+    }
     const Row w = finish(m, l, sink);
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (live) {
-        for (int j = 1; j < share; ++j) acc[i] += sums[warp + j][lane * V + i];
-        static_cast<T*>(p.o)[b * p.ob + head * p.oh + lane * V + i] = Pack<T>::from(acc[i] * w.inv);
-      }
+      if (live) static_cast<T*>(p.o)[b * p.ob + head * p.oh + lane * V + i] = Pack<T>::from(acc[i] * w.inv);
     if (p.lse && lane == 0) p.lse[(int64_t)b * p.Hq + head] = w.lse;
     return;
   }
@@ -705,17 +722,14 @@ finish_kernel(const __grid_constant__ DecodeParams p, int grid, int joins, int s
     const int slot = slot0 + i * kThreads + threadIdx.x;
     w[i] = slot < s.n && p.c.weights ? p.decay * p.c.weights[b * p.c.wb + hk * p.c.wh + slot] : 0.f;
   }
-  Span<D, ROWS> span(p, b, hk * p.tiles, p.warps ? 1 : grid);
   const int gap = (s.c0 - s.a) * kUnit;  // slots between the sinks' units and the window's
   sm100::pdl_wait();
   for (int tile = 0; tile < p.tiles; ++tile) {
     const int rows = p.G - tile * ROWS < ROWS ? p.G - tile * ROWS : ROWS, head0 = hk * p.G + tile * ROWS;
     const float* finished = p.lse + (int64_t)b * p.Hq + head0;
-    if (tile) {
-      __syncthreads();
-      if (!p.warps) span = Span<D, ROWS>(p, b, hk * p.tiles + tile, grid);
-    }
-    if (p.warps || !span.split()) {
+    if (tile) __syncthreads();
+    const Span<D, ROWS> span(p, b * vh + hk * p.tiles + tile);
+    if (!span.split()) {
       if ((int)threadIdx.x < ROWS) shared_lse[threadIdx.x] = (int)threadIdx.x < rows ? finished[threadIdx.x] : 0.f;
     } else {
       for (int r = warp; r < ROWS; r += kWarps) {
@@ -756,18 +770,15 @@ finish_kernel(const __grid_constant__ DecodeParams p, int grid, int joins, int s
 // What a call needs of the workspace, in floats each, every part a multiple of 64.
 struct Plan {
   int rows, tiles, max_units, warps, blocks;
-  size_t lse, partials, heads, scores;
+  size_t lse, partials, heads, spans, scores;
 };
 size_t round64(size_t n) { return (n + 63) & ~(size_t)63; }
 
-#ifndef V_U1
-#define V_U1 32
-#define V_U4 136
-#define V_SEQ 96
-#endif
 // Visible units up to which a (sequence, KV head) is one warp's or one block's, so that nothing is
-// left to join, where there are enough of them to fill the GPU.
-constexpr int kUnitsWarp = V_U1, kUnitsBlock = V_U4, kSeqsBlock = V_SEQ;
+// left to join, where there are enough of them to fill the GPU.  Measured with 8 KV heads of dim 64:
+// 1 x 500 slots 7.6 us by block, 7.8 dealt out; 16 x 2100 20.7 and 24; 16 x 4200 35.6 and 33.7; 24 x 4200
+// 42 and 44; 48 x 4200 66 and 76.  Longer ones are dealt out: their lengths may differ more.
+constexpr int kUnitsWarp = 32, kUnitsBlock = 136, kSeqsBlock = 96, kUnitsMany = 264, kSeqsMany = 192;
 
 Plan plan(const SwaPagedDecodeArgs& a) {
   const SwaPagedKV& c = a.cache;
@@ -786,6 +797,7 @@ Plan plan(const SwaPagedDecodeArgs& a) {
   const int most = D == 128 ? Shape<128>::kMaxBlocks : Shape<64>::kMaxBlocks;
   if (r.max_units <= kUnitsWarp) r.warps = seqs >= most ? 1 : kWarps;
   else if (r.max_units <= kUnitsBlock && seqs >= kSeqsBlock) r.warps = kWarps;
+  else if (r.max_units <= kUnitsMany && seqs >= kSeqsMany) r.warps = kWarps;
   if (r.warps) {
     r.blocks = (int)((seqs * r.warps + kWarps - 1) / kWarps);
   } else {
@@ -796,6 +808,7 @@ Plan plan(const SwaPagedDecodeArgs& a) {
   r.lse = a.weights_out && !a.lse ? round64((size_t)c.batch * a.n_q_heads) : 0;
   r.partials = r.warps ? 0 : round64(2 * part * r.blocks);
   r.heads = r.warps ? 0 : round64(kWarps * part * r.blocks);
+  r.spans = r.warps ? 0 : round64(2 * (size_t)seqs);
   r.scores = a.weights_out ? round64((size_t)seqs * r.max_units * r.rows * kUnit) : 0;
   return r;
 }
@@ -816,8 +829,7 @@ cudaError_t launch(const DecodeParams& p, const Plan& pl, cudaStream_t st) {
   const int64_t tiles = p.wout ? (slots + kWeightSlots - 1) / kWeightSlots : 0;
   const int64_t blocks = joins + tiles * p.c.n_kv_heads * p.c.batch;
   if (blocks == 0) return cudaSuccess;
-  return launch_pdl(finish_kernel<T, D, ROWS>, (unsigned)blocks, kThreads, 0, st, p, pl.blocks, (int)joins, share,
-                    (int)tiles);
+  return launch_pdl(finish_kernel<T, D, ROWS>, (unsigned)blocks, kThreads, 0, st, p, (int)joins, share, (int)tiles);
 }
 
 template <typename T, int ROWS>
@@ -834,7 +846,7 @@ cudaError_t launch_dim(int D, const DecodeParams& p, const Plan& pl, cudaStream_
 
 size_t paged_decode_workspace(const SwaPagedDecodeArgs& a) {
   const Plan r = plan(a);
-  return (r.lse + r.partials + r.heads + r.scores) * sizeof(float);
+  return (r.lse + r.partials + r.heads + r.spans + r.scores) * sizeof(float);
 }
 
 cudaError_t launch_paged_decode(const PagedParams& c, const SwaPagedDecodeArgs& a, cudaStream_t st) {
@@ -852,7 +864,8 @@ cudaError_t launch_paged_decode(const PagedParams& c, const SwaPagedDecodeArgs& 
   p.lse = a.lse ? a.lse : pl.lse ? ws : nullptr;
   p.partials = ws + pl.lse;
   p.heads = p.partials + pl.partials;
-  p.scores = pl.scores ? p.heads + pl.heads : nullptr;
+  p.spans = reinterpret_cast<int2*>(p.heads + pl.heads);
+  p.scores = pl.scores ? p.heads + pl.heads + pl.spans : nullptr;
   p.sinks = a.sink_logits;
   p.wout = a.weights_out; p.wob = a.wo_stride_b; p.woh = a.wo_stride_h;
   p.decay = a.decay;

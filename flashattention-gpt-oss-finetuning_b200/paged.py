@@ -233,15 +233,19 @@ class PagedKVCache:
         weights of this token, summed over the query heads of each KV head, in the slots in use
         (``cache.weights`` itself to accumulate in place; without cache.weights only the new ones).
         ``return_lse``: also the base-2 log-sum-exp ``[B, Hq]``."""
-        if not _rows_ok(q):
-            q = q.clone(memory_format=torch.contiguous_format)
         # numbers as numbers: a tensor's value could change under its key
-        window_size = None if window_size is None else int(window_size)
-        softmax_scale = None if softmax_scale is None else float(softmax_scale)
+        if window_size is not None:
+            window_size = int(window_size)
+        if softmax_scale is not None:
+            softmax_scale = float(softmax_scale)
         sink_size, decay = int(sink_size), float(decay)
-        key = ("decode", _form(q), window_size, sink_size, softmax_scale, _form(sinks), _form(weights_out), decay)
+        key = ("decode", q.shape, q.stride(), q.dtype, window_size, sink_size, softmax_scale, decay, _form(sinks),
+               _form(weights_out))
         block = self._calls.get(key)
-        if block is None:
+        if block is None or q.data_ptr() % 16:
+            if not _rows_ok(q):
+                q = q.clone(memory_format=torch.contiguous_format)
+                return self.decode(q, window_size, sink_size, softmax_scale, sinks, weights_out, decay, return_lse)
             block = self._calls.put(key, self._decode_block(q, window_size, sink_size, softmax_scale, sinks, weights_out, decay))
         dev = self._dev
         self._here(q, sinks, weights_out)
