@@ -63,7 +63,9 @@ int build_cache(const SwaPagedKV& c, swa::PagedParams* o) {
   if (c.table_stride < 0 || c.w_stride_b < 0 || c.w_stride_h < 0 || c.p_stride_b < 0 || c.p_stride_h < 0)
     return SWA_ERR_UNSUPPORTED;
   if (c.batch > 0) {
-    if (!c.k || !c.v || !c.page_table || !c.seq_lens) return SWA_ERR_INVALID_ARG;
+    // (a pool of no page and a table of no column need no address)
+    if ((c.n_pages > 0 && (!c.k || !c.v)) || (c.max_pages > 0 && !c.page_table) || !c.seq_lens)
+      return SWA_ERR_INVALID_ARG;
     if (!aligned16(c.k) || !aligned16(c.v)) return SWA_ERR_UNSUPPORTED;
   }
   o->k = c.k; o->v = c.v;

@@ -232,6 +232,7 @@ class PagedKVCache:
         that sees no key gives 0.  ``weights_out``: gets ``decay * cache.weights`` plus the softmax
         weights of this token, summed over the query heads of each KV head, in the slots in use
         (``cache.weights`` itself to accumulate in place; without cache.weights only the new ones).
+        It takes a workspace of 32 to 64 bytes a slot that the mask can reach and KV head.
         ``return_lse``: also the base-2 log-sum-exp ``[B, Hq]``."""
         # numbers as numbers: a tensor's value could change under its key
         if window_size is not None:

@@ -113,6 +113,8 @@ def _validate(q, k, rotary):
             raise ValueError("q and k must both be [B, H, L, D] or both be packed [T, H, D]")
         if t.dtype not in _DTYPES or t.dtype != q.dtype:
             raise TypeError(f"q and k must share one dtype in (float16, bfloat16); got {name}: {t.dtype}")
+    if _as4(q).shape[1] == 0:
+        raise ValueError("q has no heads")
     d = q.shape[-1]
     if d > 128 or d % 2 or d < rotary.dim:
         raise ValueError(f"head dimension {d} must be even, at most 128 and at least {rotary.dim}")
@@ -160,8 +162,7 @@ def rotate(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     if k is not None:
         ko = _empty(k)
         args.k.ptr, args.k_out.ptr = k.data_ptr(), ko.data_ptr()
-    if args.n_q_heads:
-        _lib.call("swa_rotary", args, dev)
+    _lib.call("swa_rotary", args, dev)
     return qo, ko
 
 
@@ -191,4 +192,6 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     strides); D even, at most 128.  ``positions`` (int32 or int64): ``[L]`` or ``[B, L]`` (packed:
     ``[T]``) for one axis, with a leading dimension of ``rotary.n_axes`` for several.  Angles
     are formed in 64 bits, so far positions lose nothing."""
-    return _Rotate.apply(q, k, positions, rotary, False)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _Rotate.apply(q, k, positions, rotary, False)
+    return rotate(q, k, positions, rotary)

@@ -164,6 +164,77 @@ def test_decode_many_sequences():
     check_decode(c, queries(c, 4, 32), window=20, sinks=2)
 
 
+@pytest.mark.parametrize("b,most,d,dtype", [(100, 2000, 32, torch.bfloat16), (200, 4200, 16, torch.float16)])
+def test_decode_a_block_a_sequence(b, most, d, dtype):
+    # lengths of which each takes a block of its own, most of them short
+    lens = [most if i % 40 == 7 else (61 * i) % 400 for i in range(b)]
+    c = Case(lens, 1, d, 64, dtype, seed=b, track=True)
+    out = torch.zeros_like(c.cache.weights)
+    check_decode(c, queries(c, 4, d), weights=out, old=c.cache.weights.cpu())
+
+
+def test_decode_without_a_table():
+    # tables of no column: every sequence is empty, or longer than its table
+    L = submodule("_lib")
+    k = torch.zeros(2, 2, 16, 64, dtype=torch.bfloat16, device=DEV)
+    table, lens = torch.zeros(3, 0, dtype=torch.int32, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV)
+    cache = pkg().PagedKVCache(k, k.clone(), table, lens)
+    q = torch.ones(3, 4, 64, dtype=torch.bfloat16, device=DEV)
+    o, lse = cache.decode(q, return_lse=True)
+    cache.check()
+    assert not o.any() and bool((lse == -math.inf).all())
+    lens[1] = 1
+    o = cache.decode(q)
+    with pytest.raises(L.SwaError):
+        cache.check()
+    assert torch.isnan(o[1].float()).all() and not o[0].any() and not o[2].any()
+    # a pool of no page: every table entry is out of range
+    none = torch.empty(0, 2, 16, 64, dtype=torch.bfloat16, device=DEV)
+    cache = pkg().PagedKVCache(none, none, torch.zeros(3, 1, dtype=torch.int32, device=DEV), lens)
+    o = cache.decode(q)
+    with pytest.raises(L.SwaError):
+        cache.check()
+    assert torch.isnan(o[1].float()).all() and not o[0].any() and not o[2].any()
+
+
+def test_books_with_strides():
+    # weights and positions as slices of wider tensors
+    c = Case([300, 77], 2, 64, 16, seed=12)
+    wide = torch.rand(2, 5, c.cap + 9, generator=c.g).to(DEV)
+    w = wide[:, 1:3, :c.cap]
+    pos = torch.arange(c.cap, dtype=torch.int32, device=DEV).repeat(2, 4, 1)[:, ::2]
+    cache = pkg().PagedKVCache(c.k, c.v, c.table, c.lens_t, weights=w, positions=pos)
+    bare = pkg().PagedKVCache(c.k.clone(), c.v.clone(), c.table, c.lens_t.clone(), weights=w.contiguous().clone(),
+                              positions=pos.contiguous().clone())
+    rest = wide.clone()
+    q = queries(c, 8, 64).to(DEV)
+    for x in (cache, bare):
+        x.decode(q, weights_out=x.weights)
+        x.evict(100, 4, 10)
+        x.check()
+    assert torch.equal(cache.weights, bare.weights) and torch.equal(cache.positions, bare.positions)
+    assert torch.equal(cache.k_pages.nan_to_num(), bare.k_pages.nan_to_num()) and cache.seq_lens.tolist() == [100, 77]
+    rest[:, 1:3, :c.cap] = w
+    assert torch.equal(wide, rest)
+
+
+def test_decode_on_two_streams_at_once():
+    c = Case([9000, 20, 5000], 2, 64, 64, seed=13, track=True)
+    qs = [queries(c, 16, 64).to(DEV) for _ in range(2)]
+    want = [(c.cache.decode(q, weights_out=w), w) for q in qs for w in [torch.zeros_like(c.cache.weights)]]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(10):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                w = torch.zeros_like(c.cache.weights)
+                got[i].append((c.cache.decode(qs[i], weights_out=w), w))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o, w in got[i]:
+            assert torch.equal(o, want[i][0]) and torch.equal(w, want[i][1])
+
+
 def test_decode_extreme_scores():
     # scores of +-thousands: one key takes all; equal scores; a scale of 0 and a negative one
     c = Case([200, 33], 2, 64, 16, torch.float16, seed=3, scale=8.0)
@@ -278,6 +349,27 @@ def test_append(even, hq, hkv, d, page, dtype):
 def check(y, x, pos, inv, axes, scale):
     from tests.test_rotary_gpu import check as same
     same(x.transpose(0, 1), y.transpose(0, 1), pos[:, None], inv, axes, False, scale)
+
+
+@pytest.mark.parametrize("b", [1024, 1025, 2500])
+def test_append_to_many_sequences(b):
+    # offsets searched in shared memory up to 1024 sequences, in global memory beyond
+    g = torch.Generator().manual_seed(b)
+    new = torch.randint(0, 4, (b,), generator=g)
+    t = int(new.sum())
+    cache = pkg().PagedKVCache.allocate(b, 1, 16, 16, 16, torch.float16, DEV)
+    old = torch.randint(0, 12, (b,), generator=g)
+    cache.seq_lens.copy_(old + new)
+    cu = torch.cat([torch.zeros(1, dtype=torch.int64), new.cumsum(0)]).to(torch.int32).to(DEV)
+    k, v = (torch.randn(t, 1, 16, generator=g).half() for _ in range(2))
+    cache.append(k.to(DEV), v.to(DEV), cu_new=cu)
+    cache.check()
+    seq = torch.repeat_interleave(torch.arange(b), new)
+    row = old[seq] + torch.arange(t) - (new.cumsum(0) - new)[seq]
+    for pages, x in ((cache.k_pages, k), (cache.v_pages, v)):
+        want = torch.zeros(b, 1, 16, 16, dtype=torch.float16)
+        want[seq, :, row] = x
+        assert torch.equal(pages.cpu(), want)
 
 
 def test_append_without_rotation_and_strides():

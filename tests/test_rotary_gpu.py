@@ -206,6 +206,36 @@ def test_empty_and_other_stream_and_graph():
     check(x.cpu(), z, pos[:, :, None] + 17, inv, [0] * 32, False, 1.0)
 
 
+def test_refusals_and_second_gradient():
+    rot = pkg().Rotary(table(32).to(DEV), sections=(16, 16))
+    q = torch.randn(1, 2, 8, 64, device=DEV, dtype=torch.float16)
+    pos = torch.zeros(2, 1, 8, dtype=torch.int64, device=DEV)
+    for bad in (pos[:1], pos[:, :, :7], pos[0], pos.cpu(), torch.zeros(2, 2, 8, dtype=torch.int64, device=DEV)):
+        with pytest.raises(ValueError):
+            pkg().apply_rotary(q, None, bad, rot)
+    with pytest.raises(TypeError):
+        pkg().apply_rotary(q, None, pos.float(), rot)
+    with pytest.raises(TypeError):
+        pkg().apply_rotary(q.float(), None, pos, rot)
+    for k in (q[:, :, :4], q[..., :32], q[0], q.cpu()):
+        with pytest.raises(ValueError):
+            pkg().apply_rotary(q, k, pos, rot)
+    for x in (q[:, :0], q[..., :32], q[..., :63]):
+        with pytest.raises(ValueError):
+            pkg().apply_rotary(x, None, pos, rot)
+    for kw in (dict(sections=(5, 5)), dict(sections=(33, -1)), dict(axes=[0] * 31), dict(axes=[0] * 32, sections=(32,)),
+               dict(axes=[300] * 32), dict(scale=float("nan"))):
+        with pytest.raises(ValueError):
+            pkg().Rotary(table(32).to(DEV), **kw)
+    # the gradient of a gradient: the map and its transpose, once more
+    x = q.clone().requires_grad_()
+    u = torch.randn_like(q).requires_grad_()
+    y, _ = pkg().apply_rotary(x, None, pos + 3, rot)
+    (g,) = torch.autograd.grad(y, x, u, create_graph=True)
+    (h,) = torch.autograd.grad(g, u, q)
+    assert torch.equal(h, y.detach())
+
+
 def test_attention_takes_the_rotation():
     g = torch.Generator().manual_seed(8)
     rot = pkg().Rotary(table(32).to(DEV), sections=(12, 10, 10))
