@@ -59,6 +59,7 @@ struct DecodeParams {
   float* wout;
   int64_t wob, woh;
   float decay;
+  int weigh_here;          // 1: decode_kernel itself writes wout
   float* partials;         // [blocks][2] Partial
   float* heads;            // [blocks][warps] Partial: the first piece of a warp that has two
   int2* spans;             // [B * Hkv * tiles]: first and last block, where dealt out
@@ -186,7 +187,7 @@ __device__ __forceinline__ Row finish(float m, float l, float sink) {
 // ---------------------------------------------------------------------------------------
 // A warp's walk over units [u0, u1) of one (sequence, KV head, tile)
 // ---------------------------------------------------------------------------------------
-template <typename T, int D, int ROWS> struct Walk {
+template <typename T, int D, int ROWS, bool WEIGH> struct Walk {
   static constexpr int kHalves = ROWS == 16 ? 2 : 1;  // rows of a thread: lane / 4 (+ 8)
   static constexpr int kNt = D / 8, kKs = D / 16, kStages = Shape<D>::kStages;
 
@@ -315,7 +316,7 @@ template <typename T, int D, int ROWS> struct Walk {
               for (int r = 0; r < kHalves; ++r) sc[j][2 * r + e] = -INFINITY;
           }
       }
-      if (p.scores) {
+      if constexpr (WEIGH) {
         float* out = p.scores + (((int64_t)b * p.c.n_kv_heads * p.tiles + hv) * p.max_units + u) * (ROWS * kUnit);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -475,6 +476,40 @@ __device__ __forceinline__ void join(const DecodeParams& p, int b, int hv, int c
   }
 }
 
+// The softmax weights on a visible slot, summed over the heads of a tile: exp2 of the stored scores
+// less the finished log-sum-exp.  Rows without a head add 0: their scores are -inf.
+template <int ROWS>
+__device__ __forceinline__ float slot_weight(const DecodeParams& p, const Sequence& s, int bh, int slot,
+                                             const float (&lse)[ROWS]) {
+  const int place = slot < s.a * kUnit ? slot : slot - (s.c0 - s.a) * kUnit;
+  const float4* sc = reinterpret_cast<const float4*>(p.scores + ((int64_t)bh * p.max_units * kUnit + place) * ROWS);
+  float sum = 0.f;
+#pragma unroll
+  for (int r = 0; r < ROWS; r += 4) {
+    const float4 x = sc[r / 4];
+    sum += (fast_exp2(x.x - lse[r]) + fast_exp2(x.y - lse[r + 1])) +
+           (fast_exp2(x.z - lse[r + 2]) + fast_exp2(x.w - lse[r + 3]));
+  }
+  return sum;
+}
+__device__ __forceinline__ float old_weight(const DecodeParams& p, int b, int h, int slot) {
+  return p.c.weights ? p.decay * p.c.weights[b * p.c.wb + h * p.c.wh + slot] : 0.f;
+}
+
+// wout of one (sequence, KV head) of one tile, by `step` threads that have its scores and its lse.
+template <int ROWS>
+__device__ __forceinline__ void weigh(const DecodeParams& p, const Sequence& s, int b, int h, int first, int step) {
+  float lse[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) lse[r] = r < p.G ? p.lse[(int64_t)b * p.Hq + h * p.G + r] : 0.f;
+#pragma unroll 4
+  for (int slot = first; slot < s.n; slot += step) {
+    float w = old_weight(p, b, h, slot);
+    if (slot < s.sinks || slot >= s.first) w += slot_weight<ROWS>(p, s, b * p.c.n_kv_heads + h, slot, lse);
+    p.wout[b * p.wob + h * p.woh + slot] = w;
+  }
+}
+
 struct Piece {
   int bh, u0, u1, units;
 };
@@ -485,7 +520,7 @@ struct Deal {
   int blocks;
 };
 
-template <typename T, int D, int ROWS>
+template <typename T, int D, int ROWS, bool WEIGH>
 __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ Piece pieces[kWarps][2];
@@ -534,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kerne
   }
   if (lane < 2) pieces[warp][lane].bh = -1;
   __syncwarp();
-  Walk<T, D, ROWS> w;
+  Walk<T, D, ROWS, WEIGH> w;
   while (todo > 0) {
     const int u1 = (int)(todo < s.units - u ? u + todo : s.units);
     if (!p.warps && lane == 0) {
@@ -560,7 +595,13 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kerne
       s = sequence(p, ++b);
     }
   }
-  if (p.warps == 1) return;
+  if (p.warps == 1) {
+    if constexpr (WEIGH) {
+      __syncwarp();
+      if (p.weigh_here) weigh<ROWS>(p, s, b, hv, lane, 32);
+    }
+    return;
+  }
   __syncthreads();
 
   if (p.warps) {  // one (sequence, KV head, tile), its pieces in the first warps' rings
@@ -572,6 +613,10 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kerne
       count += pieces[i][1].bh >= 0;
     }
     if (count) join<T, D, ROWS>(p, b, hv, count, part, nullptr);  // (none: a warp walked it whole)
+    if constexpr (WEIGH) {
+      __syncthreads();
+      if (p.weigh_here) weigh<ROWS>(p, s, b, hv, threadIdx.x, kThreads);
+    }
     return;
   }
   // join neighbouring pieces of the same (sequence, KV head, tile)
@@ -720,9 +765,8 @@ finish_kernel(const __grid_constant__ DecodeParams p, int joins, int share, int 
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int slot = slot0 + i * kThreads + threadIdx.x;
-    w[i] = slot < s.n && p.c.weights ? p.decay * p.c.weights[b * p.c.wb + hk * p.c.wh + slot] : 0.f;
+    w[i] = slot < s.n ? old_weight(p, b, hk, slot) : 0.f;
   }
-  const int gap = (s.c0 - s.a) * kUnit;  // slots between the sinks' units and the window's
   sm100::pdl_wait();
   for (int tile = 0; tile < p.tiles; ++tile) {
     const int rows = p.G - tile * ROWS < ROWS ? p.G - tile * ROWS : ROWS, head0 = hk * p.G + tile * ROWS;
@@ -740,24 +784,14 @@ finish_kernel(const __grid_constant__ DecodeParams p, int joins, int share, int 
       }
     }
     __syncthreads();
-    float lse[ROWS];  // rows without a head add 0: their scores are -inf
+    float lse[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) lse[r] = shared_lse[r];
-    const float* scores = p.scores + (((int64_t)b * vh + hk * p.tiles + tile) * p.max_units) * (ROWS * kUnit);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int slot = slot0 + i * kThreads + threadIdx.x;
-      if (slot < s.n && (slot < s.sinks || slot >= s.first)) {
-        const float4* sc = reinterpret_cast<const float4*>(scores + (int64_t)(slot < s.a * kUnit ? slot : slot - gap) * ROWS);
-        float sum = 0.f;
-#pragma unroll
-        for (int r = 0; r < ROWS; r += 4) {
-          const float4 x = sc[r / 4];
-          sum += (fast_exp2(x.x - lse[r]) + fast_exp2(x.y - lse[r + 1])) +
-                 (fast_exp2(x.z - lse[r + 2]) + fast_exp2(x.w - lse[r + 3]));
-        }
-        w[i] += sum;
-      }
+      if (slot < s.n && (slot < s.sinks || slot >= s.first))
+        w[i] += slot_weight<ROWS>(p, s, b * vh + hk * p.tiles + tile, slot, lse);
     }
   }
 #pragma unroll
@@ -769,7 +803,7 @@ finish_kernel(const __grid_constant__ DecodeParams p, int joins, int share, int 
 
 // What a call needs of the workspace, in floats each, every part a multiple of 64.
 struct Plan {
-  int rows, tiles, max_units, warps, blocks;
+  int rows, tiles, max_units, warps, blocks, weigh_here;
   size_t lse, partials, heads, spans, scores;
 };
 size_t round64(size_t n) { return (n + 63) & ~(size_t)63; }
@@ -779,6 +813,10 @@ size_t round64(size_t n) { return (n + 63) & ~(size_t)63; }
 // 1 x 500 slots 7.6 us by block, 7.8 dealt out; 16 x 2100 20.7 and 24; 16 x 4200 35.6 and 33.7; 24 x 4200
 // 42 and 44; 48 x 4200 66 and 76.  Longer ones are dealt out: their lengths may differ more.
 constexpr int kUnitsWarp = 32, kUnitsBlock = 136, kSeqsBlock = 96, kUnitsMany = 264, kSeqsMany = 192;
+// Slots of a table up to which whoever finishes a sequence writes its weights as well, instead of a
+// second kernel with a thread a slot: 8 KV heads, 4 x 250 slots 7.2 us and 8.6, 48 x 250 10.6 and 11.0,
+// 48 x 500 19.1 and 17.1; 100 x 60 by warps 7.5 and 9.0, 100 x 250 24 and 18.5.
+constexpr int kWeighBlock = 256, kWeighWarp = 64;
 
 Plan plan(const SwaPagedDecodeArgs& a) {
   const SwaPagedKV& c = a.cache;
@@ -804,6 +842,8 @@ Plan plan(const SwaPagedDecodeArgs& a) {
     const int64_t want = (seqs * r.max_units + 2 * kWarps - 1) / (2 * kWarps);
     r.blocks = (int)(want < most ? want : most);
   }
+  // whoever finishes a short sequence writes its weights too: no second kernel
+  r.weigh_here = a.weights_out && r.tiles == 1 && cap <= (r.warps == 1 ? kWeighWarp : r.warps ? kWeighBlock : 0);
   const size_t part = (size_t)r.rows * (D + 2);
   r.lse = a.weights_out && !a.lse ? round64((size_t)c.batch * a.n_q_heads) : 0;
   r.partials = r.warps ? 0 : round64(2 * part * r.blocks);
@@ -813,20 +853,26 @@ Plan plan(const SwaPagedDecodeArgs& a) {
   return r;
 }
 
+template <typename T, int D, int ROWS, bool WEIGH>
+cudaError_t launch_decode(const DecodeParams& p, int blocks, cudaStream_t st) {
+  constexpr int smem = kWarps * Shape<D>::kRing;
+  auto kern = decode_kernel<T, D, ROWS, WEIGH>;
+  cudaError_t e = allow_smem<Walk<T, D, ROWS, WEIGH>>(kern, smem);
+  if (e != cudaSuccess) return e;
+  kern<<<blocks, kThreads, smem, st>>>(p);
+  return cudaGetLastError();
+}
+
 template <typename T, int D, int ROWS>
 cudaError_t launch(const DecodeParams& p, const Plan& pl, cudaStream_t st) {
-  constexpr int smem = kWarps * Shape<D>::kRing;
-  auto kern = decode_kernel<T, D, ROWS>;
-  cudaError_t e = allow_smem<Walk<T, D, ROWS>>(kern, smem);
+  cudaError_t e = p.wout ? launch_decode<T, D, ROWS, true>(p, pl.blocks, st) : launch_decode<T, D, ROWS, false>(p, pl.blocks, st);
   if (e != cudaSuccess) return e;
-  kern<<<pl.blocks, kThreads, smem, st>>>(p);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
   // four warps a row where the rows alone do not fill the GPU and their spans are long
   const int64_t rows = (int64_t)p.c.batch * p.c.n_kv_heads * p.tiles * ROWS;
   const int share = rows <= kSms * 8 ? kWarps : 1;
   const int64_t joins = p.warps ? 0 : (rows * share + kWarps - 1) / kWarps;
   const int64_t slots = (int64_t)p.c.max_pages * p.c.page_size;
-  const int64_t tiles = p.wout ? (slots + kWeightSlots - 1) / kWeightSlots : 0;
+  const int64_t tiles = p.wout && !p.weigh_here ? (slots + kWeightSlots - 1) / kWeightSlots : 0;
   const int64_t blocks = joins + tiles * p.c.n_kv_heads * p.c.batch;
   if (blocks == 0) return cudaSuccess;
   return launch_pdl(finish_kernel<T, D, ROWS>, (unsigned)blocks, kThreads, 0, st, p, (int)joins, share, (int)tiles);
@@ -869,6 +915,7 @@ cudaError_t launch_paged_decode(const PagedParams& c, const SwaPagedDecodeArgs& 
   p.sinks = a.sink_logits;
   p.wout = a.weights_out; p.wob = a.wo_stride_b; p.woh = a.wo_stride_h;
   p.decay = a.decay;
+  p.weigh_here = pl.weigh_here;
   if (a.cache.dtype == SWA_F16)
     return pl.rows == 8 ? launch_dim<__half, 8>(a.cache.head_dim, p, pl, st) : launch_dim<__half, 16>(a.cache.head_dim, p, pl, st);
   return pl.rows == 8 ? launch_dim<__nv_bfloat16, 8>(a.cache.head_dim, p, pl, st)
