@@ -5,21 +5,26 @@
 // slots j, with the running maximum m and sum l of an online softmax.  Partial (m, l, o) of
 // disjoint sets of slots are joined exactly: (m, l, o) -> (max m, sum l 2^(m - max), ...).
 //
-// Work is cut into units of 16 slots, all of one page.  The units of all sequences and KV heads,
-// in a row, are dealt out evenly to the warps of the grid, whatever the lengths: a warp walks its
-// range, a block joins its warps' pieces in shared memory, and a sequence that lies in one block
-// is finished there; one that spans blocks leaves a partial per block for join_kernel.  The
-// device alone knows the lengths, so the host needs none.  Where no sequence can have many
-// visible slots (a window), each (sequence, KV head) has a block of its own instead and nothing
-// is left to join.
+// Work is cut into units of 16 slots, all of one page.  Where no sequence can have many visible
+// slots, a (sequence, KV head) belongs to one block or even one warp, which finishes it.  Else the
+// units of all sequences and KV heads, in a row, are dealt out evenly to the warps of the grid,
+// whatever the lengths: a warp walks its range, a block joins its warps' pieces, and a sequence that
+// spans blocks leaves a partial per block for finish_kernel.  The device alone knows the lengths, so
+// the host needs none.
 //
-// A warp keeps a ring of K and V units in shared memory filled by 16-byte cp.async.  It multiplies
-// with mma.sync m16n8k16: up to 8 (or 16) query heads of the KV head are the 16 rows, so K and V
-// are read once per group.  The operator is bound by the bytes of the cache: 8 heads of dim 64 need
-// 8 flops a byte.  (tcgen05 takes 64 or 128 rows and shared-memory operands, and a TMEM round trip
+// A warp keeps a ring of three units of K and V in shared memory, filled by 16-byte cp.async.  It
+// multiplies with mma.sync m16n8k16: up to 8 (or 16) query heads of the KV head are the 16 rows, so
+// K and V are read once per group.  The operator is bound by the bytes of the cache: 8 heads of dim 64
+// need 8 flops a byte.  (tcgen05 takes 64 or 128 rows and shared-memory operands, and a TMEM round trip
 // for the softmax of 8 rows; there is no rate to gain here.)  The weights p are multiplied as two
 // 16-bit pieces, hi + lo, so that rounding them adds 2^-18 (bf16) to a result that is rounded at
 // 2^-9: with 8 heads the lo pieces are the tile's other 8 rows and cost nothing.
+//
+// Measured on a B200 (6.56 TB/s copy), 8 KV heads of dim 64 with 8 query heads each: 32 sequences of
+// 129 to 16384 slots (542 MB) 95 us, 5.7 TB/s; 256 windows of 128 (72 MB) 17 us, 4.2 TB/s, bound by the
+// dependent steps of one short walk a warp; one window 4.8 us, all of it latency; one sequence of
+// 131072 slots with its weights (277 MB) 69 us, of which 54 the attention (268 MB, and 34 MB of scores
+// written) and 15 the weights.
 #include "sm100.cuh"
 #include "swa_host.cuh"
 #include "swa_paged.cuh"

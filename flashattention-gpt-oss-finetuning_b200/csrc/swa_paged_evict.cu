@@ -13,6 +13,9 @@
 // memory, one cluster barrier a digit.  move_kernel: a thread per 16 bytes of K and of V of a row
 // that moves, and the lengths.  What bounds the first are its dependent steps (load, four digits, two
 // counts), the second the rows, 128 or 256 scattered bytes each.
+//
+// Measured on a B200: 4 x 8 heads of 16384 to 32768 slots cut to 4096 (57 MB of rows move): select 20 us,
+// move 16; 64 x 4 heads of some 1080 slots cut to 1024: 8 and 4 us.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -303,7 +306,8 @@ __global__ void __launch_bounds__(kMoveThreads, 8) move_kernel(const __grid_cons
 }
 
 // Blocks per (sequence, KV head): as many as fit beside one another (two an SM), of no less than
-// 2048 slots each; more where a block could not keep its keys.
+// 2048 slots each; more where a block could not keep its keys.  (4 x 8 heads of 32768 slots, eviction
+// in all: 8 blocks a head 43 us, 4 46.)
 int cluster_size(const PagedParams& c) {
   const int64_t heads = (int64_t)c.batch * c.n_kv_heads, slots = (int64_t)c.max_pages * c.page_size;
   int size = 1;
