@@ -62,6 +62,10 @@ int build_cache(const SwaPagedKV& c, swa::PagedParams* o) {
     if (x < 0 || x % 8) return SWA_ERR_UNSUPPORTED;
   if (c.table_stride < 0 || c.w_stride_b < 0 || c.w_stride_h < 0 || c.p_stride_b < 0 || c.p_stride_h < 0)
     return SWA_ERR_UNSUPPORTED;
+  // books are written: no two of their rows may be one
+  const auto apart = [&](int64_t b, int64_t h) { return (b > 0 || c.batch <= 1) && (h > 0 || c.n_kv_heads <= 1); };
+  if ((c.weights && !apart(c.w_stride_b, c.w_stride_h)) || (c.positions && !apart(c.p_stride_b, c.p_stride_h)))
+    return SWA_ERR_INVALID_ARG;
   if (c.batch > 0) {
     // (a pool of no page and a table of no column need no address)
     if ((c.n_pages > 0 && (!c.k || !c.v)) || (c.max_pages > 0 && !c.page_table) || !c.seq_lens)
@@ -148,6 +152,7 @@ int swa_paged_decode(const SwaPagedDecodeArgs* a, void* stream) {
   if (!aligned16(a->o.ptr) || a->o.stride_t % 8 || a->o.stride_h % 8) return SWA_ERR_UNSUPPORTED;
   if (a->weights_out) {
     if (a->wo_stride_b < 0 || a->wo_stride_h < 0) return SWA_ERR_UNSUPPORTED;
+    if ((a->wo_stride_b == 0 && c.batch > 1) || (a->wo_stride_h == 0 && c.n_kv_heads > 1)) return SWA_ERR_INVALID_ARG;
     // a block per 512 slots of a KV head, in one grid
     if (((int64_t)c.max_pages * c.page_size / 512 + 1) * c.n_kv_heads * c.batch > INT32_MAX / 2) return SWA_ERR_UNSUPPORTED;
   }

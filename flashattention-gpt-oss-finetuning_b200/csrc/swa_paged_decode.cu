@@ -100,7 +100,7 @@ __device__ __forceinline__ Sequence sequence(const DecodeParams& p, int b) {
 }
 __device__ __forceinline__ int unit_chunk(const Sequence& s, int u) { return u < s.a ? u : u - s.a + s.c0; }
 
-// All units of all sequences, per (KV head, tile); every lane gets the sum.
+// Units, per (KV head, tile), of this lane's sequences: `per_lane` neighbouring ones.
 __device__ __forceinline__ int64_t lane_units(const DecodeParams& p, int lane, int* per_lane) {
   const int per = (p.c.batch + 31) / 32;
   *per_lane = per;
@@ -872,7 +872,8 @@ template <typename T, int D, int ROWS>
 cudaError_t launch(const DecodeParams& p, const Plan& pl, cudaStream_t st) {
   cudaError_t e = p.wout ? launch_decode<T, D, ROWS, true>(p, pl.blocks, st) : launch_decode<T, D, ROWS, false>(p, pl.blocks, st);
   if (e != cudaSuccess) return e;
-  // four warps a row where the rows alone do not fill the GPU and their spans are long
+  // four warps a row where the rows alone do not fill the GPU and their spans are long: one sequence of
+  // 2100 slots 8.8 us so, 9.8 with one warp a row; a ragged batch of 32 97 and 95
   const int64_t rows = (int64_t)p.c.batch * p.c.n_kv_heads * p.tiles * ROWS;
   const int share = rows <= kSms * 8 ? kWarps : 1;
   const int64_t joins = p.warps ? 0 : (rows * share + kWarps - 1) / kWarps;

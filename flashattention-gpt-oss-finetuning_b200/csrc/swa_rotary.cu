@@ -13,8 +13,8 @@
 // writes, so outputs may lie on their inputs.
 //
 // Measured on a B200 (6.56 TB/s copy): q and k of the GPT-OSS layer (4 x 72 heads x 4096 x 64, 302
-// MB moved) 54 us, 5.6 TB/s; 8 x 36 heads x 3000 x 128 (443 MB) 76 us, 5.8 TB/s; 14004 packed
-// prompt tokens into pages (288 MB) 57 us, 5.1 TB/s; 64 single tokens 4 us.
+// MB moved) 50 us, 6.0 TB/s; 8 x 36 heads x 3000 x 128 (443 MB) 73 us, 6.1 TB/s; 14004 packed
+// prompt tokens into pages (288 MB) 54 us, 5.3 TB/s; 64 single tokens 4 us.
 #include "swa_host.cuh"
 #include "swa_paged.cuh"
 
@@ -22,10 +22,11 @@ namespace swa {
 namespace {
 
 constexpr int kThreads = 256;
-// 8 tokens share a block and its angles: at the GPT-OSS layer 4 take 61 us, 8 54, 16 55, 32 57
+// 8 tokens share a block and its angles: at the GPT-OSS layer 4 took 61 us, 8 54, 16 55, 32 57, and a
+// prompt of 512 tokens 7.3 us with 4, 6.4 with 8
 constexpr int kMaxTokens = 8;
 // heads whose loads a thread has under way, and blocks an SM (64 registers a thread): 1 and 6 take
-// 63 us, 2 and 4 54, 3 and 3 56, 4 and 3 54
+// 63 us, 2 and 4 54, 3 and 3 56, 4 and 3 54 (50 with the first rows called for before the angles)
 constexpr int kHeadsAhead = 2;
 constexpr int kBlocksPerSm = 4;
 constexpr int kSmemSeqs = 1024;  // sequences whose offsets are searched in shared memory
@@ -100,6 +101,33 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rows_kernel(const __gr
   const int n = p.r.n_freq, t0 = blockIdx.x * p.tok;
   const int count = p.tokens - t0 < p.tok ? p.tokens - t0 : p.tok;
   const int heads0 = blockIdx.y * p.heads_block;
+  const int lane = threadIdx.x % p.lanes, tt = threadIdx.x / p.lanes % p.tok;
+  const int first = threadIdx.x / (p.lanes * p.tok), t = t0 + tt;
+  const int64_t b = APPEND ? 0 : t / p.L, l = APPEND ? t : t % p.L;
+  const bool works = first < p.heads_par && tt < count;
+  // this thread's two pieces (element offsets) and whether they turn
+  const bool self = V > 1 && p.r.interleaved, turned = lane * V < (self ? 2 * n : n);
+  int x, y;
+  if (self) {
+    x = lane * V;
+    y = x + p.lanes * V;
+  } else {
+    x = turned ? (V == 1 && p.r.interleaved ? 2 * lane : lane * V) : 2 * lane * V;
+    y = turned ? (V == 1 && p.r.interleaved ? x + 1 : x + n) : x + V;
+  }
+  // the first rows come while the angles are formed: 50 us for the layer, 52.5 without
+  if (works) {
+    const int to = heads0 + p.heads_block < p.Hq ? heads0 + p.heads_block : p.Hq;
+#pragma unroll
+    for (int i = 0; i < kHeadsAhead; ++i) {
+      const int h = heads0 + first + i * p.heads_par;
+      if (h < to) {
+        const T* in = static_cast<const T*>(p.q.in) + b * p.q.si.b + l * p.q.si.l + h * p.q.si.h;
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(in + x));
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(in + y));
+      }
+    }
+  }
 
   if constexpr (APPEND) {
     const int32_t* cu = p.cu;
@@ -141,19 +169,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rows_kernel(const __gr
   }
   __syncthreads();
 
-  const int lane = threadIdx.x % p.lanes, tt = threadIdx.x / p.lanes % p.tok;
-  const int first = threadIdx.x / (p.lanes * p.tok);
-  if (first >= p.heads_par || tt >= count) return;
-  const int t = t0 + tt;
-  const bool self = V > 1 && p.r.interleaved;
-  // this thread's two pieces (element offsets) and whether they turn
-  int x, y;
-  bool turned;
+  if (!works) return;
   float c[V], s[V];
   if (self) {
-    x = lane * V;
-    y = (lane + p.lanes) * V;
-    turned = x < 2 * n;
 #pragma unroll
     for (int j = 0; j < V / 2; ++j) {
       const float2 u = x < 2 * n ? turns[tt][x / 2 + j] : make_float2(0.f, 0.f);
@@ -161,16 +179,12 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rows_kernel(const __gr
       c[j] = u.x; s[j] = u.y; c[V / 2 + j] = w.x; s[V / 2 + j] = w.y;
     }
   } else {
-    turned = lane * V < n;
-    x = turned ? (V == 1 && p.r.interleaved ? 2 * lane : lane * V) : 2 * lane * V;
-    y = turned ? (V == 1 && p.r.interleaved ? x + 1 : x + n) : x + V;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const float2 u = turned ? turns[tt][lane * V + j] : make_float2(0.f, 0.f);
       c[j] = u.x; s[j] = u.y;
     }
   }
-  const int64_t b = APPEND ? 0 : t / p.L, l = APPEND ? t : t % p.L;
   const int heads = p.Hq + p.Hk + (APPEND ? p.Hk : 0);
   const int end = heads0 + p.heads_block < heads ? heads0 + p.heads_block : heads;
 
@@ -239,10 +253,7 @@ int piece(const RowsParams& p) {
 template <typename T, int V, bool APPEND> cudaError_t launch(RowsParams p, cudaStream_t st) {
   p.lanes = p.D / (2 * V);
   const int heads = p.Hq + p.Hk + (APPEND ? p.Hk : 0);
-  // 8 tokens share a block where there is work for several waves of blocks (contiguous runs of
-  // rows in memory, angles formed once for many heads), else 4, so that more blocks share it
-  const int64_t threads = (int64_t)p.tokens * heads * p.lanes;
-  p.tok = threads >= (int64_t)148 * 8 * kThreads * 2 ? kMaxTokens : 4;
+  p.tok = kMaxTokens;
   while (p.tok > 1 && (p.tok * p.lanes > kThreads || p.tok / 2 >= p.tokens)) p.tok /= 2;
   p.heads_par = kThreads / (p.tok * p.lanes);
   const int64_t x = (p.tokens + p.tok - 1) / p.tok;

@@ -107,6 +107,7 @@ CACHES = [
     (dict(max_pages=2**27), 2), (dict(k=None), 1), (dict(v=None), 1), (dict(page_table=None), 1), (dict(seq_lens=None), 1),
     (dict(k=PTR + 8), 2), (dict(v=PTR + 2), 2), (dict(k_stride_row=60), 2), (dict(v_stride_page=-4096), 2),
     (dict(table_stride=-1), 2), (dict(w_stride_b=-1), 2), (dict(p_stride_h=-1), 2), (dict(batch=2**30), 2),
+    (dict(w_stride_b=0), 1), (dict(p_stride_h=0), 1),
 ]
 
 
@@ -134,6 +135,7 @@ def _packed(**kw):
     ("swa_paged_decode", _decode, dict(decay=math.nan), 1), ("swa_paged_decode", _decode, dict(q=_packed(ptr=PTR + 4)), 2),
     ("swa_paged_decode", _decode, dict(q=_packed(stride_h=60)), 2), ("swa_paged_decode", _decode, dict(o=_packed(stride_t=-8)), 1),
     ("swa_paged_decode", _decode, dict(o=_packed(ptr=None)), 1), ("swa_paged_decode", _decode, dict(weights_out=PTR, wo_stride_b=-1), 2),
+    ("swa_paged_decode", _decode, dict(weights_out=PTR, wo_stride_b=256), 1),
     ("swa_paged_evict", _evict, dict(keep=0), 1), ("swa_paged_evict", _evict, dict(trigger=-1), 1),
     ("swa_paged_evict", _evict, dict(sink_size=-1), 1), ("swa_paged_evict", _evict, dict(recent=-1), 1),
     ("swa_paged_evict", _evict, dict(sink_size=9, recent=8), 1), ("swa_paged_evict", _evict, dict(recent=2**31 - 1), 1),
@@ -152,7 +154,7 @@ def test_evict_needs_weights_and_positions():
 def test_workspace_sizes():
     lib = pkg().lib()
     size = lambda **kw: lib.swa_paged_decode_workspace_size(ctypes.byref(_decode(**kw)))  # noqa: E731
-    args = _decode(weights_out=PTR, wo_stride_b=256, wo_stride_h=64)
+    args = _decode(weights_out=PTR, wo_stride_b=256, wo_stride_h=64)  # two KV heads, rows of 64 slots
     need = lib.swa_paged_decode_workspace_size(ctypes.byref(args))
     assert need >= size() and need % 256 == 0 and size(n_q_heads=7) == 0
     if need:
