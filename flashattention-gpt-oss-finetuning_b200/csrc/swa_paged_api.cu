@@ -153,8 +153,8 @@ int swa_paged_decode(const SwaPagedDecodeArgs* a, void* stream) {
   if (a->weights_out) {
     if (a->wo_stride_b < 0 || a->wo_stride_h < 0) return SWA_ERR_UNSUPPORTED;
     if ((a->wo_stride_b == 0 && c.batch > 1) || (a->wo_stride_h == 0 && c.n_kv_heads > 1)) return SWA_ERR_INVALID_ARG;
-    // a block per 512 slots of a KV head, in one grid
-    if (((int64_t)c.max_pages * c.page_size / 512 + 1) * c.n_kv_heads * c.batch > INT32_MAX / 2) return SWA_ERR_UNSUPPORTED;
+    // a block per 256 slots of a KV head, in one grid
+    if (((int64_t)c.max_pages * c.page_size / 256 + 1) * c.n_kv_heads * c.batch > INT32_MAX / 2) return SWA_ERR_UNSUPPORTED;
   }
   if (int st = check_workspace(a->workspace, a->workspace_bytes, swa_paged_decode_workspace_size(a))) return st;
   if (int st = bind_flag(&c)) return st;

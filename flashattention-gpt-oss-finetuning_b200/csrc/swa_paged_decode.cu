@@ -38,7 +38,6 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kUnit = 16;     // slots per unit
 constexpr int kSms = 148;
-constexpr int kWeightSlots = 1024;  // slots per block of finish_kernel
 
 template <int D> struct Shape {
   static constexpr int kUnitBytes = 2 * kUnit * D * 2;  // K and V
@@ -700,10 +699,10 @@ __device__ __forceinline__ void join_row(float* m, float* l, float* acc, float m
 }
 
 // After decode_kernel.  Blocks [0, joins) join the rows of sequences that span blocks, `share` warps a
-// row.  Behind them, with weights_out, blocks of kWeightSlots slots of a (sequence, KV head):
+// row.  Behind them, with weights_out, blocks of SLOTS slots of a (sequence, KV head):
 //   weights_out = decay * weights + sum over the heads of exp2(stored score - log-sum-exp),
 // with the log-sum-exp joined once more where it spans blocks, so that nothing waits for the joins.
-template <typename T, int D, int ROWS>
+template <typename T, int D, int ROWS, int SLOTS>
 __global__ void __launch_bounds__(kThreads, 8)
 finish_kernel(const __grid_constant__ DecodeParams p, int joins, int share, int weight_tiles) {
   using P = Partial<D, ROWS>;
@@ -759,12 +758,12 @@ finish_kernel(const __grid_constant__ DecodeParams p, int joins, int share, int 
   }
   const int at = blockIdx.x - joins, hk = at / weight_tiles % p.c.n_kv_heads, b = at / weight_tiles / p.c.n_kv_heads;
   const Sequence s = sequence(p, b);
-  const int slot0 = at % weight_tiles * kWeightSlots;
+  const int slot0 = at % weight_tiles * SLOTS;
   if (slot0 >= s.n) {
     sm100::pdl_wait();  // (every block waits: the grid is not over before the one that it follows)
     return;
   }
-  constexpr int kPer = kWeightSlots / kThreads;
+  constexpr int kPer = SLOTS / kThreads;
   __shared__ float shared_lse[ROWS];
   float w[kPer];
 #pragma unroll
@@ -808,7 +807,7 @@ finish_kernel(const __grid_constant__ DecodeParams p, int joins, int share, int 
 
 // What a call needs of the workspace, in floats each, every part a multiple of 64.
 struct Plan {
-  int rows, tiles, max_units, warps, blocks, weigh_here;
+  int rows, tiles, max_units, warps, blocks, weigh_here, weigh_slots;
   size_t lse, partials, heads, spans, scores;
 };
 size_t round64(size_t n) { return (n + 63) & ~(size_t)63; }
@@ -822,6 +821,11 @@ constexpr int kUnitsWarp = 32, kUnitsBlock = 136, kSeqsBlock = 96, kUnitsMany = 
 // second kernel with a thread a slot: 8 KV heads, 4 x 250 slots 7.2 us and 8.6, 48 x 250 10.6 and 11.0,
 // 48 x 500 19.1 and 17.1; 100 x 60 by warps 7.5 and 9.0, 100 x 250 24 and 18.5.
 constexpr int kWeighBlock = 256, kWeighWarp = 64;
+// Slots of a block of finish_kernel's weights: few; but many where sequences span blocks, whose
+// partials every block joins once more, and there are more than a wave of blocks or very long spans.
+// 8 KV heads: one sequence of 4200 slots 13.0 us with 256 and 15.3 with 1024, 4 of 8400 27.1 and 27.4, 4 of
+// 16000 43.1 and 41.3, one of 131072 89 and 70; 2 KV heads, 32000 slots 26.6 and 19.0.
+constexpr int kFewSlots = 256, kManySlots = 1024;
 
 Plan plan(const SwaPagedDecodeArgs& a) {
   const SwaPagedKV& c = a.cache;
@@ -849,6 +853,8 @@ Plan plan(const SwaPagedDecodeArgs& a) {
   }
   // whoever finishes a short sequence writes its weights too: no second kernel
   r.weigh_here = a.weights_out && r.tiles == 1 && cap <= (r.warps == 1 ? kWeighWarp : r.warps ? kWeighBlock : 0);
+  const int64_t weigh_blocks = (cap + kFewSlots - 1) / kFewSlots * c.batch * c.n_kv_heads;
+  r.weigh_slots = r.warps || (weigh_blocks <= 8 * kSms && r.blocks <= 128 * seqs) ? kFewSlots : kManySlots;
   const size_t part = (size_t)r.rows * (D + 2);
   r.lse = a.weights_out && !a.lse ? round64((size_t)c.batch * a.n_q_heads) : 0;
   r.partials = r.warps ? 0 : round64(2 * part * r.blocks);
@@ -878,10 +884,11 @@ cudaError_t launch(const DecodeParams& p, const Plan& pl, cudaStream_t st) {
   const int share = rows <= kSms * 8 ? kWarps : 1;
   const int64_t joins = p.warps ? 0 : (rows * share + kWarps - 1) / kWarps;
   const int64_t slots = (int64_t)p.c.max_pages * p.c.page_size;
-  const int64_t tiles = p.wout && !p.weigh_here ? (slots + kWeightSlots - 1) / kWeightSlots : 0;
+  const int64_t tiles = p.wout && !p.weigh_here ? (slots + pl.weigh_slots - 1) / pl.weigh_slots : 0;
   const int64_t blocks = joins + tiles * p.c.n_kv_heads * p.c.batch;
   if (blocks == 0) return cudaSuccess;
-  return launch_pdl(finish_kernel<T, D, ROWS>, (unsigned)blocks, kThreads, 0, st, p, (int)joins, share, (int)tiles);
+  return launch_pdl(pl.weigh_slots == kFewSlots ? finish_kernel<T, D, ROWS, kFewSlots> : finish_kernel<T, D, ROWS, kManySlots>,
+                    (unsigned)blocks, kThreads, 0, st, p, (int)joins, share, (int)tiles);
 }
 
 template <typename T, int ROWS>

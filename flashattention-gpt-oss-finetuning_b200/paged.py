@@ -25,7 +25,7 @@ import torch
 
 from . import _lib
 from .flash_attention_gpt_oss import _DTYPES, _KERNEL_HEAD_DIMS
-from .rotary import Rotary
+from .rotary import Rotary, _empty
 
 _WHOLE = 2**31 - 1
 
@@ -187,7 +187,7 @@ class PagedKVCache:
             rotary._on(self._dev, positions)
             args.r.positions = positions.data_ptr()
             if q is not None:
-                out = torch.empty(q.shape, device=self._dev, dtype=self._dtype)
+                out = _empty(q)
                 args.q.ptr, args.q_out.ptr = q.data_ptr(), out.data_ptr()
         _lib.call("swa_paged_append", args, self._dev)
         return out
@@ -252,7 +252,7 @@ class PagedKVCache:
         self._here(q, sinks, weights_out)
         block, ws_bytes, sinks_ok = block
         args = _lib.SwaPagedDecodeArgs.from_buffer_copy(block)
-        o = torch.empty(q.shape, device=dev, dtype=self._dtype)
+        o = _empty(q)
         args.q.ptr, args.o.ptr = q.data_ptr(), o.data_ptr()
         lse = None
         if return_lse:
