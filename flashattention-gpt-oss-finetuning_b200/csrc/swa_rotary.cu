@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kThreads = 256;
 // 8 tokens share a block and its angles: at the GPT-OSS layer 4 took 61 us, 8 54, 16 55, 32 57, and a
-// prompt of 512 tokens 7.3 us with 4, 6.4 with 8
+// prompt of 512 tokens 7.3 us with 4, 6.4 with 8 (5.4 with fewer blocks)
 constexpr int kMaxTokens = 8;
 // heads whose loads a thread has under way, and blocks an SM (64 registers a thread): 1 and 6 take
 // 63 us, 2 and 4 54, 3 and 3 56, 4 and 3 54 (50 with the first rows called for before the angles)
@@ -257,8 +257,9 @@ template <typename T, int V, bool APPEND> cudaError_t launch(RowsParams p, cudaS
   while (p.tok > 1 && (p.tok * p.lanes > kThreads || p.tok / 2 >= p.tokens)) p.tok /= 2;
   p.heads_par = kThreads / (p.tok * p.lanes);
   const int64_t x = (p.tokens + p.tok - 1) / p.tok;
-  // heads are divided among blocks until they fill the GPU, 8 blocks an SM
-  int64_t groups = (148 * 8 + x - 1) / x;
+  // heads are divided among blocks until every SM has one, no further: each block forms its tokens'
+  // angles anew (a prompt of 1024 tokens: 6.1 us so, 9.9 with eight blocks an SM)
+  int64_t groups = (148 + x - 1) / x;
   const int64_t most = (heads + p.heads_par - 1) / p.heads_par;
   if (groups > most) groups = most;
   if (groups < 1) groups = 1;
