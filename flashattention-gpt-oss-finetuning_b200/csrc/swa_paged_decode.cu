@@ -10,7 +10,8 @@
 // units of all sequences and KV heads, in a row, are dealt out evenly to the warps of the grid,
 // whatever the lengths: a warp walks its range, a block joins its warps' pieces, and a sequence that
 // spans blocks leaves a partial per block for finish_kernel.  The device alone knows the lengths, so
-// the host needs none.
+// the host needs none.  (More than 16 query heads a KV head are tiles of 16, each a block's, which walk
+// the same range at the same time: the cache comes from memory once.)
 //
 // A warp keeps a ring of three units of K and V in shared memory, filled by 16-byte cp.async.  It
 // multiplies with mma.sync m16n8k16: up to 8 (or 16) query heads of the KV head are the 16 rows, so
@@ -66,7 +67,7 @@ struct DecodeParams {
   int weigh_here;          // 1: decode_kernel itself writes wout
   float* partials;         // [blocks][2] Partial
   float* heads;            // [blocks][warps] Partial: the first piece of a warp that has two
-  int2* spans;             // [B * Hkv * tiles]: first and last block, where dealt out
+  int2* spans;             // [B * Hkv * tiles]: first and last group of blocks, where dealt out
   float* scores;           // [B * Hkv * tiles][max_units][16][ROWS]
 };
 
@@ -99,7 +100,7 @@ __device__ __forceinline__ Sequence sequence(const DecodeParams& p, int b) {
 }
 __device__ __forceinline__ int unit_chunk(const Sequence& s, int u) { return u < s.a ? u : u - s.a + s.c0; }
 
-// Units, per (KV head, tile), of this lane's sequences: `per_lane` neighbouring ones.
+// Units, per KV head, of this lane's sequences: `per_lane` neighbouring ones.
 __device__ __forceinline__ int64_t lane_units(const DecodeParams& p, int lane, int* per_lane) {
   const int per = (p.c.batch + 31) / 32;
   *per_lane = per;
@@ -551,23 +552,24 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kerne
   } else {
     int per;
     const int64_t mine = lane_units(p, lane, &per);
-    const int64_t total = warp_sum(mine) * vh, before = warp_prefix(mine, lane) * vh;
-    const int blocks = active_blocks(total, gridDim.x);
-    if ((int)blockIdx.x >= blocks) return;
-    const int64_t b0 = total * blockIdx.x / blocks, b1 = total * (blockIdx.x + 1) / blocks;
+    const int heads = p.c.n_kv_heads, group = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
+    const int64_t total = warp_sum(mine) * heads, before = warp_prefix(mine, lane) * heads;
+    const int blocks = active_blocks(total, gridDim.x / p.tiles);
+    if (group >= blocks) return;
+    const int64_t b0 = total * group / blocks, b1 = total * (group + 1) / blocks;
     const int64_t at = b0 + (b1 - b0) * warp / kWarps;
     todo = b0 + (b1 - b0) * (warp + 1) / kWarps - at;
     // the lane whose sequences hold `at`, then the sequence
-    const unsigned has = __ballot_sync(~0u, at >= before && at < before + mine * vh);
+    const unsigned has = __ballot_sync(~0u, at >= before && at < before + mine * heads);
     const int src = has ? __ffs(has) - 1 : 0;
     int64_t rest = at - __shfl_sync(~0u, before, src);
     b = src * per;
     s = sequence(p, b);
-    while (todo > 0 && rest >= (int64_t)s.units * vh) {
-      rest -= (int64_t)s.units * vh;
+    while (todo > 0 && rest >= (int64_t)s.units * heads) {
+      rest -= (int64_t)s.units * heads;
       s = sequence(p, ++b);
     }
-    hv = (int)(rest / s.units);
+    hv = (int)(rest / s.units) * p.tiles + tile;
     u = (int)(rest % s.units);
     if (lane == 0) deals[warp] = {at, total, blocks};
   }
@@ -579,7 +581,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kerne
     if (!p.warps && lane == 0) {
       Deal& d = deals[warp];
       // block c holds units [total c / blocks, total (c + 1) / blocks)
-      if (u == 0) p.spans[b * vh + hv] = make_int2(blockIdx.x, (int)(((d.at + s.units) * d.blocks - 1) / d.total));
+      if (u == 0)
+        p.spans[b * vh + hv] = make_int2(blockIdx.x / p.tiles, (int)(((d.at + s.units) * d.blocks - 1) / d.total));
       d.at += u1 - u;
     }
     w.run(p, saddr(ring), lane, b, hv, s, u, u1);
@@ -594,8 +597,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kerne
       if (lane == 0) pieces[warp][1] = {b * vh + hv, u, u1, s.units};
     }
     u = 0;
-    if (todo > 0 && ++hv == vh) {
-      hv = 0;
+    if (todo > 0 && (hv += p.tiles) >= vh) {  // (b and hv stay at the last one)
+      hv %= p.tiles;
       s = sequence(p, ++b);
     }
   }
@@ -653,11 +656,12 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kerne
   }
 }
 
-// The blocks that hold units of one (sequence, KV head, tile), and their partials.
+// The groups of blocks, a block for each tile, that hold units of one (sequence, KV head), and the
+// partials of one tile.
 template <int D, int ROWS> struct Span {
-  int c0, c1;
+  int c0, c1, tile, tiles;
   float* partials;
-  __device__ __forceinline__ Span(const DecodeParams& p, int bh) : partials(p.partials) {
+  __device__ __forceinline__ Span(const DecodeParams& p, int bh) : tile(bh % p.tiles), tiles(p.tiles), partials(p.partials) {
     const int2 s = p.warps ? make_int2(0, 0) : p.spans[bh];
     c0 = s.x;
     c1 = s.y;
@@ -665,7 +669,7 @@ template <int D, int ROWS> struct Span {
   __device__ __forceinline__ bool split() const { return c1 > c0; }
   // The first block's last run of units, the others' first.
   __device__ __forceinline__ float* part(int c) const {
-    return partials + ((int64_t)c * 2 + (c > c0 ? 0 : 1)) * Partial<D, ROWS>::kFloats;
+    return partials + (((int64_t)c * tiles + tile) * 2 + (c > c0 ? 0 : 1)) * Partial<D, ROWS>::kFloats;
   }
 };
 
@@ -848,8 +852,9 @@ Plan plan(const SwaPagedDecodeArgs& a) {
   if (r.warps) {
     r.blocks = (int)((seqs * r.warps + kWarps - 1) / kWarps);
   } else {
-    const int64_t want = (seqs * r.max_units + 2 * kWarps - 1) / (2 * kWarps);
-    r.blocks = (int)(want < most ? want : most);
+    const int64_t want = ((int64_t)c.batch * c.n_kv_heads * r.max_units + 2 * kWarps - 1) / (2 * kWarps);
+    const int64_t groups = most > r.tiles ? most / r.tiles : 1;
+    r.blocks = (int)(want < groups ? want : groups) * r.tiles;
   }
   // whoever finishes a short sequence writes its weights too: no second kernel
   r.weigh_here = a.weights_out && r.tiles == 1 && cap <= (r.warps == 1 ? kWeighWarp : r.warps ? kWeighBlock : 0);

@@ -149,7 +149,8 @@ def test_decode_weights(hq, hkv, d, dtype, window, sinks):
 
 
 @pytest.mark.parametrize("lens,hq,hkv,d", [([20000], 8, 1, 64), ([5000, 3, 0, 9000], 16, 2, 128), ([30000, 1], 4, 4, 16),
-                                           ([4096] * 3 + [17] * 30, 8, 2, 64), ([70000], 64, 8, 32)])
+                                           ([4096] * 3 + [17] * 30, 8, 2, 64), ([70000], 64, 8, 32),
+                                           ([9000, 3, 0, 5000], 40, 2, 64), ([30000], 40, 1, 128), ([7000, 1], 32, 2, 16)])
 def test_decode_long_and_ragged(lens, hq, hkv, d):
     c = Case(lens, hkv, d, 64, seed=lens[0], track=True)
     out = torch.zeros_like(c.cache.weights)
