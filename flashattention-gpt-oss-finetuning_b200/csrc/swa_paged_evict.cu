@@ -15,7 +15,7 @@
 // counts), the second the rows, 128 or 256 scattered bytes each.
 //
 // Measured on a B200: 4 x 8 heads of 16384 to 32768 slots cut to 4096 (57 MB of rows move): select 20 us,
-// move 16; 64 x 4 heads of some 1080 slots cut to 1024: 8 and 4 us.
+// move 16; 64 x 4 heads of some 1080 slots cut to 1024, in one kernel, 12 us.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -45,6 +45,7 @@ struct EvictParams {
   int32_t* counts;  // [batch, Hkv]: moves, -1 where the sequence is not cut
   int32_t* lists;   // [batch, Hkv, 2, most]: free slots, then the slots that fill them
   int most;         // moves that a (sequence, KV head) can have
+  int all_here;     // 1: a cluster is a sequence, a block a head, and select_kernel moves the rows itself
 };
 
 // Order-preserving map of a weight to [0x007fffff, 0xff800000]: NaN as -inf, -0 as +0.
@@ -65,12 +66,32 @@ __device__ __forceinline__ int warp_before(int x, int lane) {
   return y - x;
 }
 
+// A 16-byte piece of K and of V of slot `from` to slot `to`, with the first also weight and position.
+__device__ __forceinline__ void move_piece(const EvictParams& p, int b, int h, int to, int from, int part, bool* bad) {
+  const int pt = paged_page(p.c, b, to / p.c.page_size, bad), pf = paged_page(p.c, b, from / p.c.page_size, bad);
+  if (pt >= 0 && pf >= 0) {
+    char* k = static_cast<char*>(p.c.k) + 2 * h * p.c.kh + 16 * part;
+    char* v = static_cast<char*>(p.c.v) + 2 * h * p.c.vh + 16 * part;
+    const int rt = to % p.c.page_size, rf = from % p.c.page_size;
+    const uint4 x = *reinterpret_cast<const uint4*>(k + 2 * (pf * p.c.kp + rf * p.c.kr));
+    const uint4 y = *reinterpret_cast<const uint4*>(v + 2 * (pf * p.c.vp + rf * p.c.vr));
+    *reinterpret_cast<uint4*>(k + 2 * (pt * p.c.kp + rt * p.c.kr)) = x;
+    *reinterpret_cast<uint4*>(v + 2 * (pt * p.c.vp + rt * p.c.vr)) = y;
+  }
+  if (part == 0) {
+    float* w = p.c.weights + b * p.c.wb + h * p.c.wh;
+    int32_t* x = p.c.positions + b * p.c.pb + h * p.c.ph;
+    w[to] = w[from];
+    x[to] = x[from];
+  }
+}
+
 struct Shared {
   uint32_t hist[kDigits][kBins];
   uint32_t sent[2][kMaxCluster][kBins];  // the blocks' histograms, of even and odd digits
   int warp[kWarps][2];                   // counts of each warp
   int block[2][kMaxCluster][2];          // the blocks' counts, by round
-  int found[kDigits][3]; // digit, slots above it, slots in it
+  int found[kDigits][3];                 // digit, slots above it, slots in it
   int last_equal;                        // the last slot with key t that is kept
 };
 
@@ -87,7 +108,7 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const __grid_consta
   sm100::pdl_trigger();
   if (bad || n <= p.keep || n <= p.trigger) {  // alike for the cluster
     if (tid == 0 && rank == 0) {
-      p.counts[at] = -1;
+      if (!p.all_here) p.counts[at] = -1;
       if (bad) *p.c.page_error = 1;
     }
     return;
@@ -104,7 +125,8 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const __grid_consta
   auto key_of = [&](int s) -> uint32_t { return KEEP_KEYS ? keys[s - lo] : make_key(w[s], pos[s]); };
 
   for (int i = tid; i < kDigits * kBins; i += kThreads) (&sh.hist[0][0])[i] = 0;
-  if (cluster > 1) cl.barrier_arrive();  // waited for before the first write to another block
+  // waited for before the first write to another block, or before the sequence's new length is written
+  if (cluster > 1 || p.all_here) cl.barrier_arrive();
   __syncthreads();
   // digits from the top; `prefix` holds those found
   uint32_t prefix = 0;
@@ -267,7 +289,21 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const __grid_consta
     move0 += __popc(votes & ~below);
   }
   // the last block's last warp ends at their number
-  if (rank == cluster - 1 && warp == kWarps - 1 && lane == 0) p.counts[at] = move0;
+  if (rank == cluster - 1 && warp == kWarps - 1 && lane == 0) {
+    if (!p.all_here) p.counts[at] = move0;
+    else sh.block[0][0][0] = move0;
+  }
+  if (p.all_here) {
+    __syncthreads();
+    const int pieces = sh.block[0][0][0] << p.piece_bits;
+    for (int e = tid; e < pieces; e += kThreads) {
+      const int m = e >> p.piece_bits;
+      move_piece(p, b, h, free_list[m], move_list[m], e & (p.pieces - 1), &bad);
+    }
+    if (bad) *p.c.page_error = 1;
+    cl.barrier_wait();  // every head has read the old length
+    if (h == 0 && tid == 0) p.c.seq_lens[b] = p.keep;
+  }
 }
 
 // blockIdx.y strides over (sequence, KV head), blockIdx.x over the pieces of its moves; then the
@@ -284,23 +320,7 @@ __global__ void __launch_bounds__(kMoveThreads, 8) move_kernel(const __grid_cons
     if (moves >= 0 && h == 0 && e == 0) p.c.seq_lens[b] = p.keep;
     if (m >= moves) continue;
     const int32_t* free_list = p.lists + (int64_t)at * 2 * p.most;
-    const int to = free_list[m], from = free_list[p.most + m];
-    const int pt = paged_page(p.c, b, to / p.c.page_size, &bad), pf = paged_page(p.c, b, from / p.c.page_size, &bad);
-    if (pt >= 0 && pf >= 0) {
-      char* k = static_cast<char*>(p.c.k) + 2 * h * p.c.kh + 16 * part;
-      char* v = static_cast<char*>(p.c.v) + 2 * h * p.c.vh + 16 * part;
-      const int rt = to % p.c.page_size, rf = from % p.c.page_size;
-      const uint4 x = *reinterpret_cast<const uint4*>(k + 2 * (pf * p.c.kp + rf * p.c.kr));
-      const uint4 y = *reinterpret_cast<const uint4*>(v + 2 * (pf * p.c.vp + rf * p.c.vr));
-      *reinterpret_cast<uint4*>(k + 2 * (pt * p.c.kp + rt * p.c.kr)) = x;
-      *reinterpret_cast<uint4*>(v + 2 * (pt * p.c.vp + rt * p.c.vr)) = y;
-    }
-    if (part == 0) {
-      float* w = p.c.weights + b * p.c.wb + h * p.c.wh;
-      int32_t* x = p.c.positions + b * p.c.pb + h * p.c.ph;
-      w[to] = w[from];
-      x[to] = x[from];
-    }
+    move_piece(p, b, h, free_list[m], free_list[p.most + m], part, &bad);
   }
   if (bad) *p.c.page_error = 1;
 }
@@ -327,7 +347,7 @@ cudaError_t launch(const EvictParams& p, int cluster, int smem, cudaStream_t st)
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)cluster;
+  at[0].val.clusterDim.x = (unsigned)(p.all_here ? p.c.n_kv_heads : cluster);
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
@@ -361,9 +381,13 @@ cudaError_t launch_paged_evict(const PagedParams& c, const SwaPagedEvictArgs& a,
   p.most = (int)most_moves(a);
   const int cluster = cluster_size(c);
   const int64_t slots = (int64_t)c.max_pages * c.page_size;
+  // Few moves, at most four pieces a thread, of heads that fit in a cluster: one kernel does it all
+  // (calls one after the other: 8 heads of one sequence 12.8 us, 14.0 with two kernels; 64 x 4 heads of dim 128
+  // 22.1 and 22.6).
+  p.all_here = cluster == 1 && c.n_kv_heads <= kMaxCluster && (int64_t)p.most * p.pieces <= 4 * kThreads;
   const int64_t per = (slots + cluster * kThreads - 1) / (cluster * kThreads) * kThreads;
   cudaError_t e = per <= kMaxKeys ? launch<true>(p, cluster, (int)per * 4, st) : launch<false>(p, cluster, 0, st);
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || p.all_here) return e;
   const int64_t x = ((int64_t)p.most * p.pieces + kMoveThreads - 1) / kMoveThreads;
   const int heads = c.batch * c.n_kv_heads;
   return launch_pdl(move_kernel, dim3((unsigned)x, (unsigned)(heads < 65535 ? heads : 65535)), kMoveThreads, 0, st, p);
