@@ -425,7 +425,8 @@ def test_evict(values, keep, trigger, sinks, recent):
         assert torch.equal(got.cpu(), ref)
 
 
-@pytest.mark.parametrize("n,keep,hkv,b", [(20000, 3000, 2, 1), (9000, 8999, 1, 2), (5000, 1, 1, 1), (2049, 1024, 8, 3), (120000, 17000, 1, 1), (400000, 150000, 1, 1)])
+@pytest.mark.parametrize("n,keep,hkv,b", [(20000, 3000, 2, 1), (9000, 8999, 1, 2), (5000, 1, 1, 1), (2049, 1024, 8, 3), (120000, 17000, 1, 1), (400000, 150000, 1, 1),
+                                          (600, 300, 12, 2), (1500, 700, 4, 2)])
 def test_evict_long(n, keep, hkv, b):
     d, page = 16, 64
     lens = [n - 7 * i for i in range(b)]
