@@ -62,13 +62,6 @@ __host__ __device__ __forceinline__ VisibleSlots visible_slots(int n, int W, int
   return r;
 }
 
-template <typename T> __device__ __forceinline__ float to_f32(T x);
-template <> __device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
-template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T> __device__ __forceinline__ T from_f32(float x);
-template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-
 // cos and sin (times scale) of position * inv_freq.  The product in 64 bits: at position 2^17 a
 // 32-bit product would be off by up to 2^-8 rad; in 64 bits the angle, in turns, is exact to
 // about 2^-53 of itself, and what is left of whole turns is small enough for 32 bits.
