@@ -92,6 +92,7 @@ struct Shared {
   int warp[kWarps][2];                   // counts of each warp
   int block[2][kMaxCluster][2];          // the blocks' counts, by round
   int found[kDigits][3];                 // digit, slots above it, slots in it
+  int sums[kBins / 32];                  // counts of 32 bins each
   int last_equal;                        // the last slot with key t that is kept
 };
 
@@ -178,31 +179,29 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const __grid_consta
             reinterpret_cast<const uint4*>(hist)[part];
       cl.sync();
     }
-    if (warp == 0) {
-      // eight bins a lane, from the top
-      const int own = kBins - 8 * lane - 8;
-      int c[8] = {};
+    // a bin a thread, from the top
+    int here = 0, above = 0;
+    if (tid < kBins) {
+      const int bin = kBins - 1 - tid;
+      if (cluster > 1) {
 #pragma unroll
-      for (int r = 0; r < kMaxCluster; ++r) {
-        if (r >= cluster) break;
-        const uint32_t* other = cluster > 1 ? sh.sent[round & 1][r] : hist;
-        const uint4 x = *reinterpret_cast<const uint4*>(other + own), y = *reinterpret_cast<const uint4*>(other + own + 4);
-        c[0] += y.w; c[1] += y.z; c[2] += y.y; c[3] += y.x; c[4] += x.w; c[5] += x.z; c[6] += x.y; c[7] += x.x;
+        for (int r = 0; r < kMaxCluster; ++r)
+          if (r < cluster) here += sh.sent[round & 1][r][bin];
+      } else {
+        here = hist[bin];
       }
-      int mine = 0;
+      above = warp_before(here, lane);
+      if (lane == 31) sh.sums[warp] = above + here;
+    }
+    __syncthreads();
+    if (tid < kBins) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mine += c[i];
-      int above = warp_before(mine, lane);
-      if (above < need && above + mine >= need) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (above < need && above + c[i] >= need) {
-            sh.found[round][0] = own + 7 - i;
-            sh.found[round][1] = above;
-            sh.found[round][2] = c[i];
-          }
-          above += c[i];
-        }
+      for (int i = 0; i < kBins / 32; ++i)
+        if (i < warp) above += sh.sums[i];
+      if (above < need && above + here >= need) {  // one thread
+        sh.found[round][0] = kBins - 1 - tid;
+        sh.found[round][1] = above;
+        sh.found[round][2] = here;
       }
     }
     __syncthreads();
