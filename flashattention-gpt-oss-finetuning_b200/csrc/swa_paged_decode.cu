@@ -534,6 +534,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kBlocksPerSm) decode_kerne
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int vh = p.c.n_kv_heads * p.tiles;
   unsigned char* ring = smem + warp * Shape<D>::kRing;
+  // All earlier launches are over past the wait, and only then may finish_kernel start: it reads lengths
+  // and weights before its own wait.
+  sm100::pdl_wait();
   sm100::pdl_trigger();
 
   // this warp's range: units [u, ...) of (b, hv), `todo` of them
@@ -875,8 +878,7 @@ cudaError_t launch_decode(const DecodeParams& p, int blocks, cudaStream_t st) {
   auto kern = decode_kernel<T, D, ROWS, WEIGH>;
   cudaError_t e = allow_smem<Walk<T, D, ROWS, WEIGH>>(kern, smem);
   if (e != cudaSuccess) return e;
-  kern<<<blocks, kThreads, smem, st>>>(p);
-  return cudaGetLastError();
+  return launch_pdl(kern, (unsigned)blocks, kThreads, smem, st, p);
 }
 
 template <typename T, int D, int ROWS>

@@ -104,9 +104,10 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const __grid_consta
   const int rank = blockIdx.x % cluster, at = blockIdx.x / cluster;
   const int h = at % p.c.n_kv_heads, b = at / p.c.n_kv_heads;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  sm100::pdl_wait();
+  sm100::pdl_trigger();
   bool bad = false;
   const int n = paged_len(p.c, b, &bad);
-  sm100::pdl_trigger();
   if (bad || n <= p.keep || n <= p.trigger) {  // alike for the cluster
     if (tid == 0 && rank == 0) {
       if (!p.all_here) p.counts[at] = -1;
@@ -344,12 +345,14 @@ cudaError_t launch(const EvictParams& p, int cluster, int smem, cudaStream_t st)
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = (unsigned)(p.all_here ? p.c.n_kv_heads : cluster);
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kern, p, cluster);
 }
 

@@ -15,6 +15,7 @@
 // Measured on a B200 (6.56 TB/s copy): q and k of the GPT-OSS layer (4 x 72 heads x 4096 x 64, 302
 // MB moved) 50 us, 6.0 TB/s; 8 x 36 heads x 3000 x 128 (443 MB) 73 us, 6.1 TB/s; 14004 packed
 // prompt tokens into pages (288 MB) 54 us, 5.3 TB/s; 64 single tokens 4 us.
+#include "sm100.cuh"
 #include "swa_host.cuh"
 #include "swa_paged.cuh"
 
@@ -115,6 +116,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rows_kernel(const __gr
     x = turned ? (V == 1 && p.r.interleaved ? 2 * lane : lane * V) : 2 * lane * V;
     y = turned ? (V == 1 && p.r.interleaved ? x + 1 : x + n) : x + V;
   }
+  sm100::pdl_wait();
   // the first rows come while the angles are formed: 50 us for the layer, 52.5 without
   if (works) {
     const int to = heads0 + p.heads_block < p.Hq ? heads0 + p.heads_block : p.Hq;
@@ -265,8 +267,7 @@ template <typename T, int V, bool APPEND> cudaError_t launch(RowsParams p, cudaS
   if (groups < 1) groups = 1;
   p.heads_block = (int)((heads + groups - 1) / groups);
   const int y = (heads + p.heads_block - 1) / p.heads_block;
-  rows_kernel<T, V, APPEND><<<dim3((unsigned)x, (unsigned)y), kThreads, 0, st>>>(p);
-  return cudaGetLastError();
+  return launch_pdl(rows_kernel<T, V, APPEND>, dim3((unsigned)x, (unsigned)y), kThreads, 0, st, p);
 }
 
 template <bool APPEND> cudaError_t launch(const RowsParams& p, int dtype, cudaStream_t st) {
