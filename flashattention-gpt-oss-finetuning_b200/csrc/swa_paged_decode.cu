@@ -22,8 +22,8 @@
 // 2^-9: with 8 heads the lo pieces are the tile's other 8 rows and cost nothing.
 //
 // Measured on a B200 (6.56 TB/s copy), 8 KV heads of dim 64 with 8 query heads each: 32 sequences of
-// 129 to 16384 slots (542 MB) 95 us, 5.7 TB/s; 256 windows of 128 (72 MB) 17 us, 4.2 TB/s, bound by the
-// dependent steps of one short walk a warp; one window 4.8 us, all of it latency; one sequence of
+// 129 to 16384 slots (542 MB) 96 us, 5.7 TB/s; 256 windows of 128 (72 MB) 16 us, 4.5 TB/s, bound by the
+// dependent steps of one short walk a warp; one window 4.5 us, all of it latency; one sequence of
 // 131072 slots with its weights (277 MB) 69 us, of which 54 the attention (268 MB, and 34 MB of scores
 // written) and 15 the weights.
 #include "sm100.cuh"
