@@ -14,6 +14,10 @@
 // that moves, and the lengths.  What bounds the first are its dependent steps (load, four digits, two
 // counts), the second the rows, 128 or 256 scattered bytes each.
 //
+// A sequence with a page out of range among those in use is not cut: no row, weight or number of it
+// moves and its length stays, like one whose length is out of range.  Every block looks through the
+// sequence's whole table, so that all its heads decide alike without a word between them.
+//
 // Measured on a B200: 4 x 8 heads of 16384 to 32768 slots cut to 4096 (57 MB of rows move): select 20 us,
 // move 16; 64 x 4 heads of some 1080 slots cut to 1024, in one kernel, 12 us.
 #include <cooperative_groups.h>
@@ -67,17 +71,18 @@ __device__ __forceinline__ int warp_before(int x, int lane) {
 }
 
 // A 16-byte piece of K and of V of slot `from` to slot `to`, with the first also weight and position.
-__device__ __forceinline__ void move_piece(const EvictParams& p, int b, int h, int to, int from, int part, bool* bad) {
-  const int pt = paged_page(p.c, b, to / p.c.page_size, bad), pf = paged_page(p.c, b, from / p.c.page_size, bad);
-  if (pt >= 0 && pf >= 0) {
-    char* k = static_cast<char*>(p.c.k) + 2 * h * p.c.kh + 16 * part;
-    char* v = static_cast<char*>(p.c.v) + 2 * h * p.c.vh + 16 * part;
-    const int rt = to % p.c.page_size, rf = from % p.c.page_size;
-    const uint4 x = *reinterpret_cast<const uint4*>(k + 2 * (pf * p.c.kp + rf * p.c.kr));
-    const uint4 y = *reinterpret_cast<const uint4*>(v + 2 * (pf * p.c.vp + rf * p.c.vr));
-    *reinterpret_cast<uint4*>(k + 2 * (pt * p.c.kp + rt * p.c.kr)) = x;
-    *reinterpret_cast<uint4*>(v + 2 * (pt * p.c.vp + rt * p.c.vr)) = y;
-  }
+// (select_kernel has found both pages in range; one that is not, in a table written meanwhile, is not followed.)
+__device__ __forceinline__ void move_piece(const EvictParams& p, int b, int h, int to, int from, int part) {
+  bool bad = false;
+  const int pt = paged_page(p.c, b, to / p.c.page_size, &bad), pf = paged_page(p.c, b, from / p.c.page_size, &bad);
+  if (bad) return;
+  char* k = static_cast<char*>(p.c.k) + 2 * h * p.c.kh + 16 * part;
+  char* v = static_cast<char*>(p.c.v) + 2 * h * p.c.vh + 16 * part;
+  const int rt = to % p.c.page_size, rf = from % p.c.page_size;
+  const uint4 x = *reinterpret_cast<const uint4*>(k + 2 * (pf * p.c.kp + rf * p.c.kr));
+  const uint4 y = *reinterpret_cast<const uint4*>(v + 2 * (pf * p.c.vp + rf * p.c.vr));
+  *reinterpret_cast<uint4*>(k + 2 * (pt * p.c.kp + rt * p.c.kr)) = x;
+  *reinterpret_cast<uint4*>(v + 2 * (pt * p.c.vp + rt * p.c.vr)) = y;
   if (part == 0) {
     float* w = p.c.weights + b * p.c.wb + h * p.c.wh;
     int32_t* x = p.c.positions + b * p.c.pb + h * p.c.ph;
@@ -126,6 +131,11 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const __grid_consta
   auto make_key = [&](float weight, int x) -> uint32_t { return x < p.sink || x >= late ? 0xffffffffu : weight_key(weight); };
   auto key_of = [&](int s) -> uint32_t { return KEEP_KEYS ? keys[s - lo] : make_key(w[s], pos[s]); };
 
+  // the pages in use, all of them; the first one's number arrives while the weights are read
+  const int32_t* table = p.c.table + (int64_t)b * p.c.table_stride;
+  const int pages = (n - 1) / p.c.page_size + 1;
+  const unsigned first_page = tid < pages ? (unsigned)table[tid] : 0u;
+
   for (int i = tid; i < kDigits * kBins; i += kThreads) (&sh.hist[0][0])[i] = 0;
   // waited for before the first write to another block, or before the sequence's new length is written
   if (cluster > 1 || p.all_here) cl.barrier_arrive();
@@ -162,6 +172,9 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const __grid_consta
           if (base + 32 * i < whi) count(s < whi, key);
         }
       }
+      bad = tid < pages && first_page >= (unsigned)p.c.n_pages;
+      for (int i = tid + kThreads; i < pages; i += kThreads) paged_page(p.c, b, i, &bad);
+      bad = __syncthreads_or(bad);
     } else {
       for (int base = wlo; base < whi; base += 32) {
         const int s = base + lane;
@@ -169,8 +182,8 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const __grid_consta
         const bool counts = s < whi && key >> (shift + 8) == prefix;
         if (__any_sync(~0u, counts)) count(counts, key);
       }
+      __syncthreads();
     }
-    __syncthreads();
     if (cluster > 1) {
       // 16 bytes of the histogram to a block by each thread
       const int to = tid / (kBins / 4), part = tid % (kBins / 4);
@@ -290,19 +303,19 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const __grid_consta
   }
   // the last block's last warp ends at their number
   if (rank == cluster - 1 && warp == kWarps - 1 && lane == 0) {
-    if (!p.all_here) p.counts[at] = move0;
-    else sh.block[0][0][0] = move0;
+    if (bad) *p.c.page_error = 1;
+    if (!p.all_here) p.counts[at] = bad ? -1 : move0;
+    else sh.block[0][0][0] = bad ? 0 : move0;
   }
   if (p.all_here) {
     __syncthreads();
     const int pieces = sh.block[0][0][0] << p.piece_bits;
     for (int e = tid; e < pieces; e += kThreads) {
       const int m = e >> p.piece_bits;
-      move_piece(p, b, h, free_list[m], move_list[m], e & (p.pieces - 1), &bad);
+      move_piece(p, b, h, free_list[m], move_list[m], e & (p.pieces - 1));
     }
-    if (bad) *p.c.page_error = 1;
     cl.barrier_wait();  // every head has read the old length
-    if (h == 0 && tid == 0) p.c.seq_lens[b] = p.keep;
+    if (h == 0 && tid == 0 && !bad) p.c.seq_lens[b] = p.keep;
   }
 }
 
@@ -311,7 +324,6 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const __grid_consta
 // 57 MB move (18 us, 3.2 TB/s in scattered rows of 128 bytes).
 __global__ void __launch_bounds__(kMoveThreads, 8) move_kernel(const __grid_constant__ EvictParams p) {
   sm100::pdl_wait();
-  bool bad = false;
   const int heads = p.c.batch * p.c.n_kv_heads;
   const int64_t e = (int64_t)blockIdx.x * kMoveThreads + threadIdx.x;
   const int m = (int)(e >> p.piece_bits), part = (int)e & (p.pieces - 1);
@@ -320,9 +332,8 @@ __global__ void __launch_bounds__(kMoveThreads, 8) move_kernel(const __grid_cons
     if (moves >= 0 && h == 0 && e == 0) p.c.seq_lens[b] = p.keep;
     if (m >= moves) continue;
     const int32_t* free_list = p.lists + (int64_t)at * 2 * p.most;
-    move_piece(p, b, h, free_list[m], free_list[p.most + m], part, &bad);
+    move_piece(p, b, h, free_list[m], free_list[p.most + m], part);
   }
-  if (bad) *p.c.page_error = 1;
 }
 
 // Blocks per (sequence, KV head): as many as fit beside one another (two an SM), of no less than

@@ -247,8 +247,11 @@ SWA_API int swa_rotary(const SwaRotaryArgs* args, void* stream);
  * slots are in use.  All integer arrays are DEVICE arrays: no call reads them on the host.
  * Table entries behind a sequence's last page are not read.  An entry outside [0, n_pages) or
  * a length above max_pages * page_size that a call meets is never followed: rows of such pages
- * are neither read nor written, the sequence's attention output is NaN, and a following
- * swa_check_device returns SWA_ERR_BAD_PAGE.  A negative length counts as 0.
+ * are neither read nor written, the sequence's attention output is NaN, an eviction leaves the
+ * sequence as it is, all heads of it alike, and a following swa_check_device returns
+ * SWA_ERR_BAD_PAGE.  (An append writes those of its tokens whose own page is in range; an
+ * eviction meets the entries of all pages in use of the sequences that it would cut.)  A
+ * negative length counts as 0.
  * ------------------------------------------------------------------------------------ */
 typedef struct SwaPagedKV {
   void* k;                     /* [n_pages, n_kv_heads, page_size, D], D contiguous        */

@@ -628,3 +628,41 @@ def test_serving_run():
         decode(y)
         if step % 4 == 3:
             evict()
+
+
+@pytest.mark.parametrize("lens,keep,hkv,d", [([90, 90, 90, 90, 90, 60], 50, 2, 64), ([400] * 6, 200, 12, 16), ([6000] * 5 + [5000], 2100, 1, 32),
+                                             ([30000] * 6, 4000, 2, 16)], ids=["one-kernel", "two-kernels", "clusters-2", "clusters"])
+def test_an_eviction_leaves_a_bad_sequence_alone(lens, keep, hkv, d):
+    L = submodule("_lib")
+    c = Case(lens, hkv, d, 16, seed=22, track=True, room=40)
+    used, page0 = -(-lens[0] // 16), int(c.table[0, 0])
+    c.table[0, 0], c.table[1, keep // 16 + 1], c.table[2, used - 1] = -1, c.k.shape[0], 2**31 - 1
+    lens_t = c.lens_t.tolist()
+    lens_t[3] = c.cap + 1
+    c.lens_t.copy_(torch.tensor(lens_t, dtype=torch.int32))
+    c.table[4, used], c.table[4, used + 1] = -5, c.k.shape[0] + 9  # behind its last page: nothing of it
+    bits = lambda x: x.cpu().view(torch.int16 if x.dtype == torch.bfloat16 else torch.int32).clone()  # noqa: E731
+    k, v, w, pos = before = [bits(x) for x in (c.k, c.v, c.cache.weights, c.cache.positions)]
+    k, v, w, pos = (x.clone() for x in (k, v, w, pos))
+    c.cache.evict(keep, 2, 10)
+    with pytest.raises(L.SwaError) as e:
+        c.cache.check()
+    assert e.value.status == L.SWA_ERR_BAD_PAGE
+    table = c.table.cpu()
+    for i in (4, 5):
+        for x in range(hkv):
+            free, movers = orc.evict(before[2][i, x].view(torch.float32), before[3][i, x], lens[i], lens[i], keep, 2, 10)
+            assert free
+            for to, fr in zip(free, movers):
+                for pool, old in ((k, before[0]), (v, before[1])):
+                    pool[table[i, to // 16], x, to % 16] = old[table[i, fr // 16], x, fr % 16]
+                w[i, x, to], pos[i, x, to] = before[2][i, x, fr], before[3][i, x, fr]
+    assert c.lens_t.tolist() == lens_t[:4] + [keep, keep]
+    for got, ref in ((c.k, k), (c.v, v), (c.cache.weights, w), (c.cache.positions, pos)):
+        assert torch.equal(bits(got), ref)
+    # a bad page mended: the same call again cuts its sequence too
+    c.table[0, 0] = page0
+    c.cache.evict(keep, 2, 10)
+    with pytest.raises(L.SwaError):
+        c.cache.check()
+    assert c.lens_t.tolist() == [keep] + lens_t[1:4] + [keep, keep]
