@@ -176,6 +176,18 @@ template <int D> __device__ __forceinline__ uint32_t swizzled(int row, int piece
   return (uint32_t)(row * kPieces + (piece ^ x)) * 16;
 }
 
+// A sequence with a page or a length out of range: its partials' maximum is NaN (a score's NaN never gets into
+// a maximum, only into sums), and its log-sum-exp this one, which no arithmetic yields; whoever writes
+// weights leaves those of such a sequence alone.
+__device__ __forceinline__ float bad_lse() { return __uint_as_float(0xffc0bad0u); }
+__device__ __forceinline__ bool is_bad(float lse) { return __float_as_uint(lse) == 0xffc0bad0u; }
+// The larger one; NaN where one of them is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // A finished row's output and log-sum-exp from its joined maximum, sum and value.
 struct Row {
   float inv, lse;
@@ -185,7 +197,7 @@ __device__ __forceinline__ Row finish(float m, float l, float sink) {
   const float f = fast_exp2(m - base), total = l * f + fast_exp2(sink - base);
   Row r;
   r.inv = total == 0.f ? 0.f : f / total;
-  r.lse = total == 0.f ? -INFINITY : top + log2f(total);
+  r.lse = m != m ? bad_lse() : total == 0.f ? -INFINITY : top + log2f(total);
   return r;
 }
 
@@ -398,7 +410,7 @@ template <typename T, int D, int ROWS, bool WEIGH> struct Walk {
     for (int r = 0; r < kHalves; ++r) {
       l[r] += __shfl_xor_sync(~0u, l[r], 1);
       l[r] += __shfl_xor_sync(~0u, l[r], 2);
-      if (bad) l[r] = NAN;
+      if (bad) m[r] = l[r] = NAN;
     }
     if (kHalves == 1)
 #pragma unroll
@@ -453,7 +465,7 @@ __device__ __forceinline__ void join(const DecodeParams& p, int b, int hv, int c
 #pragma unroll
     for (int i = 0; i < kMost; ++i) {
       m[i] = i < count ? P::m(part[i])[r] : -INFINITY;
-      top = fmaxf(top, m[i]);
+      top = max_nan(top, m[i]);
     }
     const float base = top == -INFINITY ? 0.f : top;
     float l = 0.f, x = 0.f, y = 0.f;
@@ -507,6 +519,7 @@ __device__ __forceinline__ void weigh(const DecodeParams& p, const Sequence& s, 
   float lse[ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) lse[r] = r < p.G ? p.lse[(int64_t)b * p.Hq + h * p.G + r] : 0.f;
+  if (is_bad(lse[0])) return;
 #pragma unroll 4
   for (int slot = first; slot < s.n; slot += step) {
     float w = old_weight(p, b, h, slot);
@@ -682,12 +695,12 @@ __device__ __forceinline__ void span_stats(const Span<D, ROWS>& s, int r, int la
   using P = Partial<D, ROWS>;
   float mm = -INFINITY, ll = 0.f;
   for (int c = s.c0 + lane; c <= s.c1; c += 32) {
-    const float x = P::m(s.part(c))[r], y = P::l(s.part(c))[r], up = fmaxf(mm, x), base = up == -INFINITY ? 0.f : up;
+    const float x = P::m(s.part(c))[r], y = P::l(s.part(c))[r], up = max_nan(mm, x), base = up == -INFINITY ? 0.f : up;
     ll = ll * fast_exp2(mm - base) + y * fast_exp2(x - base);
     mm = up;
   }
   float top = mm;
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  for (int o = 16; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(~0u, top, o));
   ll *= fast_exp2(mm - (top == -INFINITY ? 0.f : top));
   for (int o = 16; o; o >>= 1) ll += __shfl_xor_sync(~0u, ll, o);
   *m = top;
@@ -697,7 +710,7 @@ __device__ __forceinline__ void span_stats(const Span<D, ROWS>& s, int r, int la
 // Adds partial (mi, li, oi) of a row to (m, l, acc).
 template <int V>
 __device__ __forceinline__ void join_row(float* m, float* l, float* acc, float mi, float li, const float* oi) {
-  const float up = fmaxf(*m, mi), base = up == -INFINITY ? 0.f : up;
+  const float up = max_nan(*m, mi), base = up == -INFINITY ? 0.f : up;
   const float f = fast_exp2(*m - base), g = fast_exp2(mi - base);
   *m = up;
   *l = *l * f + li * g;
@@ -805,6 +818,7 @@ finish_kernel(const __grid_constant__ DecodeParams p, int joins, int share, int 
         w[i] += slot_weight<ROWS>(p, s, b * vh + hk * p.tiles + tile, slot, lse);
     }
   }
+  if (is_bad(shared_lse[0])) return;  // (all tiles are, or none)
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int slot = slot0 + i * kThreads + threadIdx.x;

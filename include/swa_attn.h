@@ -304,7 +304,8 @@ typedef struct SwaPagedDecodeArgs {
 /* Attention of one new token per sequence over its cache: slot j < n = seq_lens[b] is visible
  * iff n - 1 - j < window_size or j < sink_size.  lse as in swa_fwd.  With weights_out:
  *   weights_out[b, h, j] = decay * cache.weights[b, h, j] + sum over the query heads of KV
- * head h of their softmax weight on slot j (0 where it is not visible), for j < n. */
+ * head h of their softmax weight on slot j (0 where it is not visible), for j < n.  Rows of a
+ * sequence with a page or a length out of range are left as they are. */
 SWA_API int swa_paged_decode(const SwaPagedDecodeArgs* args, void* stream);
 
 /* Scratch that swa_paged_decode needs, by the sizes, the window and the sinks (of the pointers

@@ -666,3 +666,44 @@ def test_an_eviction_leaves_a_bad_sequence_alone(lens, keep, hkv, d):
     with pytest.raises(L.SwaError):
         c.cache.check()
     assert c.lens_t.tolist() == [keep] + lens_t[1:4] + [keep, keep]
+
+
+WEIGH_PATHS = [
+    # lens, hq, hkv, d: by a warp with its weights, by a warp, by a block with its weights, by a block,
+    # dealt out, dealt out in tiles of query heads, a block a sequence of long ones
+    ([1 + (i * 7) % 60 for i in range(620)], 4, 1, 16), ([1 + (i * 7) % 200 for i in range(620)], 12, 1, 32),
+    ([90, 200, 150, 33], 8, 2, 64), ([500, 40, 300, 77], 16, 2, 128), ([9000, 200, 5000, 7000], 16, 2, 64),
+    ([3000, 200, 700, 90], 40, 2, 64), ([2100 if i % 20 == 3 else 90 for i in range(100)], 4, 1, 64),
+]
+
+
+@pytest.mark.parametrize("lens,hq,hkv,d", WEIGH_PATHS, ids=[f"{len(x[0])}x{max(x[0])}x{x[1]}" for x in WEIGH_PATHS])
+def test_weights_of_a_bad_sequence_are_left_alone(lens, hq, hkv, d):
+    L = submodule("_lib")
+    c = Case(lens, hkv, d, 16, seed=21, track=True)
+    q = queries(c, hq, d)
+    q[2, 0, 0] = math.nan               # a NaN of the model's is one: its sequence's weights are NaN
+    first, last = 0, len(lens) - 1
+    c.table[first, (lens[first] - 1) // 16] = c.k.shape[0]  # on the last page in use
+    lens_t = c.lens_t.tolist()
+    lens_t[last] = c.cap + 1
+    c.lens_t.copy_(torch.tensor(lens_t, dtype=torch.int32))
+    old = c.cache.weights.cpu().clone()
+    for out in (torch.full_like(c.cache.weights, 5.0), c.cache.weights):
+        before = out.cpu().clone()
+        o, lse = c.cache.decode(q.to(DEV), weights_out=out, return_lse=True)
+        with pytest.raises(L.SwaError):
+            c.cache.check()
+        got = out.cpu()
+        for i in (first, last):
+            assert torch.isnan(o[i].float()).all() and torch.isnan(lse[i]).all()
+            assert torch.equal(got[i], before[i])
+        assert torch.isnan(o[2, 0].float()).all() and torch.isnan(got[2, 0, :lens[2]]).all()
+        for i in range(1, last):
+            ro, _, p, amount, delta = orc.decode(q[i], *c.rows[i], lens[i], WHOLE, 0)
+            for h in range(1 if i == 2 else 0, hkv):
+                rows = slice(h * (hq // hkv), (h + 1) * (hq // hkv))
+                add, rel = p[rows].sum(0), relative(d, lens[i], delta[rows]).max()
+                ref = old[i, h, :lens[i]].double() + add
+                assert bool(((got[i, h, :lens[i]].double() - ref).abs() <= add * rel + 2.0**-22 * (2 * ref + add)).all()), (i, h)
+            assert torch.equal(got[i, :, lens[i]:], before[i, :, lens[i]:])
