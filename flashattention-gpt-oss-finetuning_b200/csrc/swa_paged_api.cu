@@ -178,6 +178,8 @@ int swa_paged_evict(const SwaPagedEvictArgs* a, void* stream) {
   // nothing can be longer than the budget
   if (a->keep >= (int64_t)c.max_pages * c.page_size) return SWA_OK;
   if (int st = check_workspace(a->workspace, a->workspace_bytes, swa_paged_evict_workspace_size(a))) return st;
+  // token numbers go by a count that evictions do not shorten
+  if (!a->cache.seen || a->cache.seen == a->cache.seq_lens) return SWA_ERR_INVALID_ARG;
   if (int st = bind_flag(&c)) return st;
   return swa::host_record(swa::launch_paged_evict(c, *a, static_cast<cudaStream_t>(stream)));
 }

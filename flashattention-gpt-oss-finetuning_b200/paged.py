@@ -57,7 +57,9 @@ class PagedKVCache:
     behind a sequence's last page are not read.  For eviction also ``weights`` (fp32) and
     ``positions`` (int32), ``[B, Hkv, max_pages * page_size]``: the attention that each slot has
     had and the number of its token; and ``seen`` (int32 ``[B]``): tokens so far, which evictions
-    leave as it is (``seq_lens`` when omitted).
+    leave as it is.  Without ``seen``, ``seq_lens`` counts the tokens: that holds until the first
+    eviction shortens it, so such a cache is evicted once and refuses a second time.  Caches that
+    are evicted do not share ``seq_lens``: the first one's eviction would cut the others unselected.
 
     The tensors are the caller's: their values may change between calls (also under a captured
     graph), the cache itself holds only their addresses.  A page number outside the pool or a
@@ -102,6 +104,8 @@ class PagedKVCache:
         for name, t in (("seq_lens", seq_lens), ("seen", seen)):
             if t is not None and (t.shape != (b,) or (b > 1 and t.stride(0) != 1)):
                 raise ValueError(f"{name} must be [{b}], contiguous")
+        if b and seen is not None and seen.data_ptr() == seq_lens.data_ptr():
+            raise ValueError("seen must not be seq_lens itself, which evictions shorten")
         self._t = (k_pages, v_pages, page_table, seq_lens, weights, positions, seen)
         self._dev, self._dtype = k_pages.device, k_pages.dtype
         self._b, self._hkv, self._d, self._cap = b, hkv, d, m * page
@@ -112,6 +116,7 @@ class PagedKVCache:
                                   ptr(positions), *st(weights), *st(positions), n, page, m, b, hkv, d,
                                   _DTYPES[k_pages.dtype])
         self._calls = _lib.Calls()
+        self._cut = False  # evicted without a count of tokens
 
     @classmethod
     def allocate(cls, batch: int, n_kv_heads: int, head_dim: int, max_len: int, page_size: int = 64,
@@ -304,7 +309,9 @@ class PagedKVCache:
         those of the largest ``weights`` (ties: the lowest slot).  Kept slots below ``keep`` stay
         where they are, and the others, in order, fill the places that came free, so the order of
         slots is no longer that of tokens: attend with ``window_size=None`` afterwards.
-        ``seq_lens`` becomes ``keep``.  Pages of a sequence that is cut must be its own."""
+        ``seq_lens`` becomes ``keep``.  Pages of a sequence that is cut must be its own.  More than one
+        eviction, or a captured one, needs a cache with ``seen``.  Weights are what ``decode`` has
+        added: those of a prompt are 0 after its append, which leaves its lowest slots."""
         keep, sink_size, recent = int(keep), int(sink_size), int(recent)
         trigger = keep if trigger is None else int(trigger)
         key = ("evict", keep, sink_size, recent, trigger)
@@ -315,9 +322,17 @@ class PagedKVCache:
         if block is None:
             return
         args = _lib.SwaPagedEvictArgs.from_buffer_copy(block)
+        seen = self.seen
+        if seen is None:
+            with torch.cuda.device(self._dev):
+                if self._cut or torch.cuda.is_current_stream_capturing():
+                    raise ValueError("a cache without seen can be evicted once: seq_lens no longer counts its tokens")
+                seen = self.seq_lens.clone()
+            args.cache.seen = seen.data_ptr()
         ws = torch.empty(ws_bytes, device=self._dev, dtype=torch.uint8)
         args.workspace, args.workspace_bytes = ws.data_ptr(), ws_bytes
         _lib.call("swa_paged_evict", args, self._dev)
+        self._cut = self.seen is None
 
     def _evict_block(self, keep, sink_size, recent, trigger):
         """The argument block of an eviction (None: no sequence can be that long) and the bytes of

@@ -260,8 +260,10 @@ typedef struct SwaPagedKV {
   int64_t v_stride_page, v_stride_head, v_stride_row;
   const int32_t* page_table;   /* [batch, max_pages], row stride table_stride              */
   int64_t table_stride;
-  int32_t* seq_lens;           /* [batch]; written by swa_paged_evict alone                */
-  const int32_t* seen;         /* [batch] tokens seen so far, or NULL: seq_lens            */
+  int32_t* seq_lens;           /* [batch]; written by swa_paged_evict alone: caches that it
+                                  cuts do not share it                                     */
+  const int32_t* seen;         /* [batch] tokens seen so far; NULL: seq_lens, which holds
+                                  until the first eviction                                 */
   float* weights;              /* [batch, n_kv_heads, max_pages * page_size], or NULL      */
   int32_t* positions;          /* same shape: the token number of each slot, or NULL       */
   int64_t w_stride_b, w_stride_h, p_stride_b, p_stride_h; /* elements                      */
@@ -313,7 +315,7 @@ SWA_API int swa_paged_decode(const SwaPagedDecodeArgs* args, void* stream);
 SWA_API size_t swa_paged_decode_workspace_size(const SwaPagedDecodeArgs* args);
 
 typedef struct SwaPagedEvictArgs {
-  SwaPagedKV cache;            /* weights and positions given                              */
+  SwaPagedKV cache;            /* weights, positions and seen given, seen not seq_lens     */
   int32_t keep;                /* slots left to a sequence that is cut                     */
   int32_t trigger;             /* sequences with more slots than max(trigger, keep) are cut */
   int32_t sink_size;           /* tokens numbered below it are held ...                    */

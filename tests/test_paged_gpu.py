@@ -707,3 +707,39 @@ def test_weights_of_a_bad_sequence_are_left_alone(lens, hq, hkv, d):
                 ref = old[i, h, :lens[i]].double() + add
                 assert bool(((got[i, h, :lens[i]].double() - ref).abs() <= add * rel + 2.0**-22 * (2 * ref + add)).all()), (i, h)
             assert torch.equal(got[i, :, lens[i]:], before[i, :, lens[i]:])
+
+
+def test_evictions_without_seen():
+    c = Case([300, 100], 2, 32, 16, torch.float16, seed=23, track=True, room=200)
+    c.cache.weights.zero_()
+    new = [torch.randn(2, 2, 32, generator=c.g).half().to(DEV) for _ in range(2)]
+    kw = dict(weights=c.cache.weights, positions=c.cache.positions)
+    with pytest.raises(ValueError):      # counted twice by advance, and shortened by an eviction
+        pkg().PagedKVCache(c.k, c.v, c.table, c.lens_t, seen=c.lens_t, **kw)
+    # with seen: a second eviction goes by the tokens' numbers
+    for step in range(3):
+        c.cache.evict(100, recent=1)
+        c.cache.advance()
+        c.cache.append(*new)
+    c.cache.evict(100, recent=1)
+    c.cache.check()
+    # zero weights: the lowest slots are kept, and the newest token in the place of the last one
+    assert c.cache.seen.tolist() == [303, 103] and c.lens_t.tolist() == [100, 100]
+    assert c.cache.positions[:, :, 99].tolist() == [[302, 302], [102, 102]]
+    # without: one eviction, before which slots are numbered as tokens
+    bare = pkg().PagedKVCache(c.k, c.v, c.table, c.lens_t.fill_(300), **kw)
+    bare.positions.copy_(torch.arange(c.cap, dtype=torch.int32))
+    bare.evict(10**9)                    # more than the table holds: nothing to cut
+    with pytest.raises(ValueError):      # a captured one is run again and again
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            bare.evict(100, recent=7)
+    bare.evict(100, recent=7)
+    bare.check()
+    assert bare.seq_lens.tolist() == [100, 100] and bare.positions[:, :, 93:100].tolist() == [[list(range(293, 300))] * 2] * 2
+    bare.advance()
+    bare.append(*new)
+    assert torch.isfinite(bare.decode(torch.ones(2, 4, 32, dtype=torch.float16, device=DEV))[0]).all()  # (all its slots were filled)
+    with pytest.raises(ValueError):
+        bare.evict(100, recent=7)
+    bare.check()
+    assert bare.seq_lens.tolist() == [101, 101]

@@ -248,3 +248,8 @@ def test_oracle_eviction():
     assert orc.evict(w, range(8), 8, 8, 4, 0, 0) == ([1, 2], [4, 6])
     # held: the first token and the last
     assert orc.evict(w, range(8), 8, 8, 4, 2, 1) == ([2, 3], [6, 7])
+
+
+def test_evict_needs_a_count_of_tokens():
+    assert _status("swa_paged_evict", _evict()) == 1                 # without seen: seq_lens, which it shortens
+    assert _status("swa_paged_evict", _evict(_cache(seen=PTR))) == 1  # seq_lens itself
