@@ -120,10 +120,11 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const __grid_consta
     }
     return;
   }
-  // this block's slots [lo, hi), a warp's [wlo, whi)
-  const int per = (n + cluster * kThreads - 1) / (cluster * kThreads) * kThreads;
+  // this block's slots [lo, hi), a warp's [wlo, whi); sums that can pass 2^31 in 64 bits (n may reach 2^31 - 1025,
+  // and 8 blocks' stretches then end at 2^31)
+  const int per = (int)(((int64_t)n + cluster * kThreads - 1) / (cluster * kThreads)) * kThreads;
   const int lo = rank * per;
-  const int wlo = lo + warp * (per / kWarps), whi = min(n, wlo + per / kWarps);
+  const int wlo = lo + warp * (per / kWarps), whi = (int)min((int64_t)n, (int64_t)wlo + per / kWarps);
 
   const float* w = p.c.weights + b * p.c.wb + h * p.c.wh;
   const int32_t* pos = p.c.positions + b * p.c.pb + h * p.c.ph;

@@ -743,3 +743,21 @@ def test_evictions_without_seen():
         bare.evict(100, recent=7)
     bare.check()
     assert bare.seq_lens.tolist() == [101, 101]
+
+
+def test_evict_next_to_two_to_the_31():
+    # the longest sequence that there can be: 2^31 - 2048 slots, of pages that are all one (no row is compared)
+    page, m = 2048, 2**20 - 1
+    n = page * m
+    k = torch.zeros(1, 1, page, 16, dtype=torch.float16, device=DEV)
+    table, lens = torch.zeros(1, m, dtype=torch.int32, device=DEV), torch.tensor([n], dtype=torch.int32, device=DEV)
+    w, pos = torch.zeros(1, 1, n, device=DEV), torch.full((1, 1, n), 5, dtype=torch.int32, device=DEV)
+    places = [0, 7, 2**28, 2**30 + 12345, n - 4097, n - 2, n - 1]
+    for i, x in enumerate(places):
+        w[0, 0, x], pos[0, 0, x] = 1.0 + i, 100 + i
+    cache = pkg().PagedKVCache(k, k.clone(), table, lens, weights=w, positions=pos, seen=lens.clone())
+    cache.evict(8)
+    cache.check()
+    # slots 0 and 7 stay, slot 1 is the lowest of the others, and 2 to 6 take the rest in order
+    assert lens.tolist() == [8] and pos[0, 0, :8].tolist() == [100, 5, 102, 103, 104, 105, 106, 101]
+    assert w[0, 0, :8].tolist() == [1.0, 0.0, 3.0, 4.0, 5.0, 6.0, 7.0, 2.0]
