@@ -493,6 +493,10 @@ __device__ __forceinline__ void join(const DecodeParams& p, int b, int hv, int c
   }
 }
 
+// What a row's scores are taken from for its weights: the log-sum-exp; 0 for one whose scores are all -inf,
+// so that it adds 0 and not NaN, as its output is 0.
+__device__ __forceinline__ float weight_base(float lse) { return lse == -INFINITY ? 0.f : lse; }
+
 // The softmax weights on a visible slot, summed over the heads of a tile: exp2 of the stored scores
 // less the finished log-sum-exp.  Rows without a head add 0: their scores are -inf.
 template <int ROWS>
@@ -518,7 +522,7 @@ template <int ROWS>
 __device__ __forceinline__ void weigh(const DecodeParams& p, const Sequence& s, int b, int h, int first, int step) {
   float lse[ROWS];
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) lse[r] = r < p.G ? p.lse[(int64_t)b * p.Hq + h * p.G + r] : 0.f;
+  for (int r = 0; r < ROWS; ++r) lse[r] = r < p.G ? weight_base(p.lse[(int64_t)b * p.Hq + h * p.G + r]) : 0.f;
   if (is_bad(lse[0])) return;
 #pragma unroll 4
   for (int slot = first; slot < s.n; slot += step) {
@@ -798,13 +802,13 @@ finish_kernel(const __grid_constant__ DecodeParams p, int joins, int share, int 
     if (tile) __syncthreads();
     const Span<D, ROWS> span(p, b * vh + hk * p.tiles + tile);
     if (!span.split()) {
-      if ((int)threadIdx.x < ROWS) shared_lse[threadIdx.x] = (int)threadIdx.x < rows ? finished[threadIdx.x] : 0.f;
+      if ((int)threadIdx.x < ROWS) shared_lse[threadIdx.x] = (int)threadIdx.x < rows ? weight_base(finished[threadIdx.x]) : 0.f;
     } else {
       for (int r = warp; r < ROWS; r += kWarps) {
         float m = -INFINITY, l = 0.f;
         if (r < rows) span_stats(span, r, lane, &m, &l);
         if (lane == 0)
-          shared_lse[r] = r < rows ? finish(m, l, p.sinks ? p.sinks[head0 + r] * kLog2e : -INFINITY).lse : 0.f;
+          shared_lse[r] = r < rows ? weight_base(finish(m, l, p.sinks ? p.sinks[head0 + r] * kLog2e : -INFINITY).lse) : 0.f;
       }
     }
     __syncthreads();

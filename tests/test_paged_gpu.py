@@ -761,3 +761,23 @@ def test_evict_next_to_two_to_the_31():
     # slots 0 and 7 stay, slot 1 is the lowest of the others, and 2 to 6 take the rest in order
     assert lens.tolist() == [8] and pos[0, 0, :8].tolist() == [100, 5, 102, 103, 104, 105, 106, 101]
     assert w[0, 0, :8].tolist() == [1.0, 0.0, 3.0, 4.0, 5.0, 6.0, 7.0, 2.0]
+
+
+def test_weights_of_rows_whose_scores_are_all_minus_infinity():
+    # like a row that sees no key: its output is 0, its log-sum-exp -inf, and it adds 0 to the weights
+    for n, hq in ((40, 8), (500, 8), (500, 20), (6000, 8)):
+        c = Case([n, n], 1, 64, 16, seed=24, track=True)
+        q = torch.zeros(2, hq, 64, dtype=torch.bfloat16)
+        q[:, :, 0] = 1.0
+        q[1, 1:, 0] = 0.25
+        c.k[c.table[0, :-(-n // 16)].long(), :, :, 0] = -math.inf
+        old = c.cache.weights.cpu().clone()
+        o, lse = c.cache.decode(q.to(DEV), weights_out=c.cache.weights, decay=0.5, return_lse=True)
+        c.cache.check()
+        got = c.cache.weights.cpu()
+        assert not o[0].any() and bool((lse[0] == -math.inf).all()) and torch.isfinite(lse[1]).all()
+        assert torch.equal(got[0, :, :n], 0.5 * old[0, :, :n])
+        assert abs(float((got[1, :, :n].double() - 0.5 * old[1, :, :n].double()).sum()) - hq) < 1e-3 * hq
+        # with a sink logit it has a sum
+        o, lse = c.cache.decode(q.to(DEV), weights_out=c.cache.weights, sinks=torch.ones(hq, device=DEV), return_lse=True)
+        assert not o[0].any() and torch.allclose(lse[0].cpu(), torch.full((hq,), 1 / math.log(2))) and torch.equal(c.cache.weights[0].cpu(), got[0])
