@@ -13,6 +13,7 @@ import ctypes
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib
 from .flash_attention_gpt_oss import _DTYPES
@@ -170,6 +171,7 @@ class _Rotate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, rotary, inverse):
         ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
         ctx.rotary, ctx.inverse, ctx.dtype = rotary, inverse, q.dtype
         return rotate(q, k, positions, rotary, inverse)
 
@@ -178,20 +180,32 @@ class _Rotate(torch.autograd.Function):
         (positions,) = ctx.saved_tensors
         dq = dq.to(ctx.dtype)
         dk = None if dk is None else dk.to(ctx.dtype)
-        # (the gradient of a gradient: only where one is asked for)
-        turn = _Rotate.apply if torch.is_grad_enabled() else rotate
-        dq, dk = turn(dq, dk, positions, ctx.rotary, not ctx.inverse)
+        dq, dk = _turn(dq, dk, positions, ctx.rotary, not ctx.inverse)
         return dq, dk, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        (positions,) = ctx.saved_tensors
+        if tq is None:
+            return None, _turn(tk, None, positions, ctx.rotary, ctx.inverse)[0]
+        return _turn(tq, tk, positions, ctx.rotary, ctx.inverse)
+
+
+def _turn(q, k, positions, rotary, inverse):
+    """Rotate, differentiably (in both modes) where a derivative is asked for."""
+    for t in (q, k):
+        if t is not None and ((torch.is_grad_enabled() and t.requires_grad) or unpack_dual(t).tangent is not None):
+            return _Rotate.apply(q, k, positions, rotary, inverse)
+    return rotate(q, k, positions, rotary, inverse)
 
 
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
                  rotary: Rotary):
-    """Rotate q and k (``k`` may be None) by their tokens' positions; differentiable.
+    """Rotate q and k (``k`` may be None) by their tokens' positions; differentiable in reverse and
+    in forward mode.
 
     q ``[B, Hq, L, D]`` and k ``[B, Hkv, L, D]``, or packed ``[T, H, D]`` (fp16 or bf16, any
     strides); D even, at most 128.  ``positions`` (int32 or int64): ``[L]`` or ``[B, L]`` (packed:
     ``[T]``) for one axis, with a leading dimension of ``rotary.n_axes`` for several.  Angles
     are formed in 64 bits, so far positions lose nothing."""
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _Rotate.apply(q, k, positions, rotary, False)
-    return rotate(q, k, positions, rotary)
+    return _turn(q, k, positions, rotary, False)

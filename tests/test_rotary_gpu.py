@@ -252,3 +252,37 @@ def test_attention_takes_the_rotation():
     flat = pos.reshape(3, 300)
     o = pkg().flash_swda_with_sink_varlen(pack(q), pack(k), pack(v), [0, 150, 300], 40, 4, rotary=rot, positions=flat)
     assert torch.equal(o.view(2, 150, 8, 64).transpose(1, 2), ref)
+
+
+def test_forward_mode_derivatives():
+    fw = torch.autograd.forward_ad
+    rot = pkg().Rotary(table(32).to(DEV), scale=1.5)
+    pos = torch.arange(9, device=DEV) + 100
+    q, k, u, w = (torch.randn(1, h, 9, 64, device=DEV).half() for h in (4, 2, 4, 2))
+    turn = submodule("rotary").rotate
+    want, values = turn(u, w, pos, rot), turn(q, k, pos, rot)
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad), fw.dual_level():
+            # both, one of them, and a leaf of a backward pass too
+            for du, dw in ((u, w), (u, None), (None, w)):
+                a = q if du is None else fw.make_dual(q.clone().requires_grad_(grad), du)
+                b = k if dw is None else fw.make_dual(k, dw)
+                ys = pkg().apply_rotary(a, b, pos, rot)
+                for y, value, tangent, ref in zip(ys, values, (du, dw), want):
+                    y = fw.unpack_dual(y)
+                    assert torch.equal(y.primal, value)
+                    if tangent is not None:
+                        assert torch.equal(y.tangent, ref)
+                    else:
+                        assert y.tangent is None or not y.tangent.any()
+            y, none = pkg().apply_rotary(fw.make_dual(q, u), None, pos, rot)
+            assert none is None and torch.equal(fw.unpack_dual(y).tangent, want[0])
+    # the attention has no forward mode and says so
+    with fw.dual_level(), pytest.raises(RuntimeError):
+        pkg().flash_swda_with_sink(fw.make_dual(q, u), k, k, 4, rotary=rot, positions=pos)
+    # a tangent through the backward pass
+    x = q.clone().requires_grad_()
+    y, _ = pkg().apply_rotary(x, None, pos, rot)
+    with fw.dual_level():
+        (g,) = torch.autograd.grad(y, x, fw.make_dual(torch.zeros_like(q), u))
+        assert torch.equal(fw.unpack_dual(g).tangent, turn(u, None, pos, rot, inverse=True)[0])
