@@ -249,6 +249,7 @@ class PagedKVCache:
                _form(weights_out))
         block = self._calls.get(key)
         if block is None or q.data_ptr() % 16:
+            self._tokens("q", q)  # rows of another width may never be aligned
             if not _rows_ok(q):
                 q = q.clone(memory_format=torch.contiguous_format)
                 return self.decode(q, window_size, sink_size, softmax_scale, sinks, weights_out, decay, return_lse)
@@ -275,9 +276,8 @@ class PagedKVCache:
         return (o, lse) if return_lse else o
 
     def _decode_block(self, q, window_size, sink_size, softmax_scale, sinks, weights_out, decay):
-        """The argument block of an attention of this form, without addresses; the bytes of its
-        workspace; whether the sink logits can be read as they are."""
-        self._tokens("q", q)
+        """The argument block of an attention of this form (q's has been looked at), without addresses; the
+        bytes of its workspace; whether the sink logits can be read as they are."""
         hq = q.shape[1]
         if q.shape[0] != self._b:
             raise ValueError(f"q must hold one token for each of {self._b} sequences; got {q.shape[0]}")

@@ -253,3 +253,23 @@ def test_oracle_eviction():
 def test_evict_needs_a_count_of_tokens():
     assert _status("swa_paged_evict", _evict()) == 1                 # without seen: seq_lens, which it shortens
     assert _status("swa_paged_evict", _evict(_cache(seen=PTR))) == 1  # seq_lens itself
+
+
+def _bare_cache(d=64):
+    """A cache object over CPU tensors, for what is refused before the library is called."""
+    P = submodule("paged")
+    L = submodule("_lib")
+    c = P.PagedKVCache.__new__(P.PagedKVCache)
+    k = torch.zeros(4, 2, 16, d, dtype=torch.bfloat16)
+    c._t = (k, k, torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), None, None, None)
+    c._dev, c._dtype, c._b, c._hkv, c._d, c._cap = k.device, k.dtype, 3, 2, d, 32
+    c._c, c._calls = _cache(batch=3, max_pages=2), L.Calls()
+    return c
+
+
+@pytest.mark.parametrize("shape", [(3, 16, 20), (3, 16, 63), (3, 16, 48), (3, 16, 8), (3, 16), (3, 1, 16, 64)])
+def test_queries_of_another_shape_are_refused(shape):
+    with pytest.raises(ValueError):
+        _bare_cache().decode(torch.zeros(shape, dtype=torch.bfloat16))
+    with pytest.raises(TypeError):
+        _bare_cache().decode(torch.zeros(3, 16, 64, dtype=torch.float16))
