@@ -178,17 +178,15 @@ class _Rotate(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dq, dk):
         (positions,) = ctx.saved_tensors
-        dq = dq.to(ctx.dtype)
-        dk = None if dk is None else dk.to(ctx.dtype)
-        dq, dk = _turn(dq, dk, positions, ctx.rotary, not ctx.inverse)
-        return dq, dk, None, None, None
+        # only the gradients that are asked for: a frozen q or k costs nothing
+        dq, dk = (d.to(ctx.dtype) if d is not None and asked else None for d, asked in
+                  zip((dq, dk), ctx.needs_input_grad))
+        return *_turn_given(dq, dk, positions, ctx.rotary, not ctx.inverse), None, None, None
 
     @staticmethod
     def jvp(ctx, tq, tk, *_):
         (positions,) = ctx.saved_tensors
-        if tq is None:
-            return None, _turn(tk, None, positions, ctx.rotary, ctx.inverse)[0]
-        return _turn(tq, tk, positions, ctx.rotary, ctx.inverse)
+        return _turn_given(tq, tk, positions, ctx.rotary, ctx.inverse)
 
 
 def _turn(q, k, positions, rotary, inverse):
@@ -197,6 +195,13 @@ def _turn(q, k, positions, rotary, inverse):
         if t is not None and ((torch.is_grad_enabled() and t.requires_grad) or unpack_dual(t).tangent is not None):
             return _Rotate.apply(q, k, positions, rotary, inverse)
     return rotate(q, k, positions, rotary, inverse)
+
+
+def _turn_given(q, k, positions, rotary, inverse):
+    """_turn of what is not None of q and k."""
+    if q is not None:
+        return _turn(q, k, positions, rotary, inverse)
+    return None, None if k is None else _turn(k, None, positions, rotary, inverse)[0]
 
 
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,

@@ -286,3 +286,27 @@ def test_forward_mode_derivatives():
     with fw.dual_level():
         (g,) = torch.autograd.grad(y, x, fw.make_dual(torch.zeros_like(q), u))
         assert torch.equal(fw.unpack_dual(g).tangent, turn(u, None, pos, rot, inverse=True)[0])
+
+
+def test_gradients_that_nobody_asks_for(monkeypatch):
+    R = submodule("rotary")
+    rot = pkg().Rotary(table(32).to(DEV))
+    pos = torch.arange(9, device=DEV)
+    q, k, dq, dk = (torch.randn(1, h, 9, 64, device=DEV).half() for h in (4, 2, 4, 2))
+    refs = R.rotate(dq, dk, pos, rot, inverse=True)
+    turned = []
+    plain = R.rotate
+
+    def counted(a, b, *rest, **kw):
+        turned.append([x.shape[1] for x in (a, b) if x is not None])
+        return plain(a, b, *rest, **kw)
+
+    monkeypatch.setattr(R, "rotate", counted)
+    for a, b, heads in ((1, 0, [4]), (0, 1, [2]), (1, 1, [4, 2])):
+        x, z = q.clone().requires_grad_(bool(a)), k.clone().requires_grad_(bool(b))
+        ys = R.apply_rotary(x, z, pos, rot)
+        turned.clear()
+        torch.autograd.backward(ys, (dq, dk))
+        assert turned == [heads]
+        assert (x.grad is None) == (not a) and (z.grad is None) == (not b)
+        assert all(y.grad is None or torch.equal(y.grad, ref) for y, ref in zip((x, z), refs))
