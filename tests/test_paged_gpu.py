@@ -781,3 +781,51 @@ def test_weights_of_rows_whose_scores_are_all_minus_infinity():
         # with a sink logit it has a sum
         o, lse = c.cache.decode(q.to(DEV), weights_out=c.cache.weights, sinks=torch.ones(hq, device=DEV), return_lse=True)
         assert not o[0].any() and torch.allclose(lse[0].cpu(), torch.full((hq,), 1 / math.log(2))) and torch.equal(c.cache.weights[0].cpu(), got[0])
+
+
+@pytest.mark.parametrize("most,d,hq", [(64, 32, 4), (211, 32, 11), (60, 128, 3), (200, 128, 8)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (20, 2)])
+def test_weights_of_many_sequences(most, d, hq, window, sinks):
+    # a warp a sequence, which writes the weights itself (tables of up to 64 slots) or leaves them to a second kernel
+    lens = [(37 * i) % (most + 1) for i in range(620)]
+    live = None if window is None else lambda n: orc.visible(n, window, sinks)  # noqa: E731
+    c = Case(lens, 1, d, 16, torch.float16, seed=most, track=True, live=live)
+    out = torch.full_like(c.cache.weights, 3.0)
+    old = c.cache.weights.cpu()
+    check_decode(c, queries(c, hq, d), window, sinks, weights=out, decay=0.75, old=old)
+    check_decode(c, queries(c, hq, d), window, sinks, logits=torch.randn(hq, generator=c.g), weights=c.cache.weights, old=old)
+
+
+@pytest.mark.parametrize("lens,keep,hkv", [([120, 64, 131], 96, 2), ([4000, 9000, 100], 3000, 2)], ids=["one-kernel", "clusters"])
+def test_evictions_in_a_graph(lens, keep, hkv):
+    # a step with its eviction, captured on its first call, replayed and mixed with eager ones
+    c = Case(lens, hkv, 32, 16, seed=26, track=True, room=40)
+    q, k, v = (torch.randn(3, h, 32, generator=c.g).bfloat16().to(DEV) for h in (4, hkv, hkv))
+    state = [c.k, c.v, c.cache.weights, c.cache.positions, c.lens_t, c.cache.seen]
+    start = [x.clone() for x in state]
+
+    def step():
+        c.cache.advance()
+        c.cache.append(k, v)
+        o = c.cache.decode(q, weights_out=c.cache.weights)
+        c.cache.evict(keep, 2, 20, keep + 4)
+        return o
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    got = []
+    for i in range(12):
+        if i % 4 == 3:
+            got.append(step().clone())
+        else:
+            graph.replay()
+            got.append(out.clone())
+    end = [x.clone() for x in state]
+    for x, y in zip(state, start):
+        x.copy_(y)
+    want = [step().clone() for _ in range(12)]
+    c.cache.check()
+    assert c.cache.seen.tolist() == [n + 12 for n in lens] and max(c.lens_t.tolist()) <= keep + 4
+    for x, y in zip(got + end, want + state):
+        assert torch.equal(x.nan_to_num(), y.nan_to_num())

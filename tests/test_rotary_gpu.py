@@ -310,3 +310,19 @@ def test_gradients_that_nobody_asks_for(monkeypatch):
         assert turned == [heads]
         assert (x.grad is None) == (not a) and (z.grad is None) == (not b)
         assert all(y.grad is None or torch.equal(y.grad, ref) for y, ref in zip((x, z), refs))
+
+
+def test_gradient_in_a_graph():
+    rot = pkg().Rotary(table(32).to(DEV))
+    pos = torch.arange(40, device=DEV)
+    q, dq = (torch.randn(1, 4, 40, 64, device=DEV).half() for _ in range(2))
+    x = q.clone().requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, _ = pkg().apply_rotary(x, None, pos, rot)
+        (g,) = torch.autograd.grad(y, x, dq)
+    pos.add_(1000)
+    dq.mul_(2)
+    graph.replay()
+    turn = submodule("rotary").rotate
+    assert torch.equal(y.detach(), turn(q, None, pos, rot)[0]) and torch.equal(g, turn(dq, None, pos, rot, inverse=True)[0])
