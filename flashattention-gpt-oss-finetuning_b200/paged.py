@@ -116,7 +116,7 @@ class PagedKVCache:
                                   ptr(positions), *st(weights), *st(positions), n, page, m, b, hkv, d,
                                   _DTYPES[k_pages.dtype])
         self._calls = _lib.Calls()
-        self._cut = False  # evicted without a count of tokens
+        self._cut = False  # evicted before
 
     @classmethod
     def allocate(cls, batch: int, n_kv_heads: int, head_dim: int, max_len: int, page_size: int = 64,
@@ -322,8 +322,7 @@ class PagedKVCache:
         if block is None:
             return
         args = _lib.SwaPagedEvictArgs.from_buffer_copy(block)
-        seen = self.seen
-        if seen is None:
+        if self._t[6] is None:
             with torch.cuda.device(self._dev):
                 if self._cut or torch.cuda.is_current_stream_capturing():
                     raise ValueError("a cache without seen can be evicted once: seq_lens no longer counts its tokens")
@@ -332,7 +331,7 @@ class PagedKVCache:
         ws = torch.empty(ws_bytes, device=self._dev, dtype=torch.uint8)
         args.workspace, args.workspace_bytes = ws.data_ptr(), ws_bytes
         _lib.call("swa_paged_evict", args, self._dev)
-        self._cut = self.seen is None
+        self._cut = True
 
     def _evict_block(self, keep, sink_size, recent, trigger):
         """The argument block of an eviction (None: no sequence can be that long) and the bytes of
