@@ -149,7 +149,10 @@ class PagedKVCache:
             self.seen.add_(n)
 
     def check(self):
-        """Synchronise, and raise if a call met a page number or a length out of range."""
+        """Wait for the current stream, and raise if a call met a page number or a length out of range.
+
+        The flag is the device's, not the cache's: it tells of any cache's calls since the last check
+        (or ``swa_check_device``), which clears it, on other streams as far as they have got."""
         with torch.cuda.device(self._dev):
             _lib.check(_lib.lib().swa_check_device(torch.cuda.current_stream().cuda_stream), "PagedKVCache")
 
@@ -171,7 +174,9 @@ class PagedKVCache:
         """Write new tokens, ``k``, ``v`` ``[T, Hkv, D]``, behind their sequences.
 
         ``seq_lens`` (and ``seen``) already count them (:meth:`advance`).  ``cu_new``: int32
-        ``[B + 1]`` CUDA offsets of each sequence's tokens; omitted, every sequence has T / B.
+        ``[B + 1]`` CUDA offsets of each sequence's tokens; omitted, every sequence has T / B.  A token
+        before the first offset or behind the last is no sequence's: it is written to no page, and
+        :meth:`check` raises.
         With ``rotary`` and ``positions`` (``[T]``, or ``[axes, T]``), k is rotated on the way, and
         so is ``q`` ``[T, Hq, D]``, which is returned."""
         k = k if k.stride(-1) == 1 else k.contiguous()
@@ -237,7 +242,8 @@ class PagedKVCache:
         that sees no key gives 0.  ``weights_out``: gets ``decay * cache.weights`` plus the softmax
         weights of this token, summed over the query heads of each KV head, in the slots in use
         (``cache.weights`` itself to accumulate in place; without cache.weights only the new ones).
-        It takes a workspace of 32 to 64 bytes a slot that the mask can reach and KV head.
+        It takes a workspace of 32 bytes (more than 8 query heads a KV head: 64 for each 16 of them) a
+        slot that the mask can reach and KV head.
         ``return_lse``: also the base-2 log-sum-exp ``[B, Hq]``."""
         # numbers as numbers: a tensor's value could change under its key
         if window_size is not None:

@@ -285,7 +285,8 @@ typedef struct SwaPagedAppendArgs {
 
 /* Write new tokens into the cache, rotating k (and q) on the way.  Token i of sequence b goes
  * to slot seq_lens[b] - new_b + i; its weight becomes 0 and its position the token number
- * seen[b] - new_b + i (where those arrays are given). */
+ * seen[b] - new_b + i (where those arrays are given).  A token before the first of cu_new's offsets
+ * or behind the last is no sequence's: it is written to no page and reported like a bad one. */
 SWA_API int swa_paged_append(const SwaPagedAppendArgs* args, void* stream);
 
 typedef struct SwaPagedDecodeArgs {
@@ -355,8 +356,9 @@ SWA_API int swa_bwd_no_alloc(const SwaBwdArgs* args, void* stream);
  *
  * Synchronise `stream`, then report (and clear) the current device's on-device error flag:
  * SWA_ERR_DEVICE_TIMEOUT if a bounded wait inside a kernel gave up since the last check
- * (that launch's outputs are then undefined), SWA_ERR_BAD_PAGE if a paged call met a page or a
- * length out of range, SWA_OK otherwise. */
+ * (that launch's outputs are then undefined), SWA_ERR_BAD_PAGE if a paged call, on whichever cache
+ * or stream of the device, met a page or a length out of range (a timeout is reported first, the
+ * page by the next call), SWA_OK otherwise. */
 SWA_API int swa_check_device(void* stream);
 
 /* Enqueue on `stream` a copy of the current device's on-device error flag into

@@ -829,3 +829,28 @@ def test_evictions_in_a_graph(lens, keep, hkv):
     assert c.cache.seen.tolist() == [n + 12 for n in lens] and max(c.lens_t.tolist()) <= keep + 4
     for x, y in zip(got + end, want + state):
         assert torch.equal(x.nan_to_num(), y.nan_to_num())
+
+
+def test_tokens_that_no_sequence_takes():
+    # offsets that end before the tokens do, or begin behind the first: those are written nowhere, and reported
+    L = submodule("_lib")
+    for cu in ([0, 3, 5], [2, 2, 7]):
+        c = Case([10, 20], 2, 32, 16, seed=25, track=True, room=8)
+        k, v = (torch.randn(7, 2, 32, generator=c.g).bfloat16() for _ in range(2))
+        q = torch.randn(7, 4, 32, generator=c.g).bfloat16().to(DEV)
+        rot = pkg().Rotary(torch.ones(16, device=DEV))
+        pos = torch.arange(7, device=DEV)
+        want = [x.cpu().view(torch.int16).clone() for x in (c.k, c.v)]
+        turned = submodule("rotary").rotate(q, k.to(DEV), pos, rot)
+        c.cache.advance(torch.tensor([cu[1] - cu[0], cu[2] - cu[1]], dtype=torch.int32, device=DEV))
+        y = c.cache.append(k.to(DEV), v.to(DEV), torch.tensor(cu, dtype=torch.int32, device=DEV), q, pos, rot)
+        with pytest.raises(L.SwaError):
+            c.cache.check()
+        assert torch.equal(y, turned[0])
+        table = c.table.cpu()
+        for b, n in enumerate((10, 20)):
+            for i in range(cu[b], cu[b + 1]):
+                slot = n + i - cu[b]
+                for x, rows in zip(want, (turned[1].cpu(), v)):
+                    x[table[b, slot // 16], :, slot % 16] = rows[i].view(torch.int16)
+        assert all(torch.equal(x.cpu().view(torch.int16), y) for x, y in zip((c.k, c.v), want))
