@@ -11,7 +11,7 @@
 // whatever the lengths: a warp walks its range, a block joins its warps' pieces, and a sequence that
 // spans blocks leaves a partial per block for finish_kernel.  The device alone knows the lengths, so
 // the host needs none.  (More than 16 query heads a KV head are tiles of 16, each a block's, which walk
-// the same range at the same time: the cache comes from memory once.)
+// the same range at the same time: every tile copies K and V to its SM, from DRAM they come once.)
 //
 // A warp keeps a ring of three units of K and V in shared memory, filled by 16-byte cp.async.  It
 // multiplies with mma.sync m16n8k16: up to 8 (or 16) query heads of the KV head are the 16 rows, so
@@ -21,7 +21,7 @@
 // 16-bit pieces, hi + lo, so that rounding them adds 2^-18 (bf16) to a result that is rounded at
 // 2^-9: with 8 heads the lo pieces are the tile's other 8 rows and cost nothing.
 //
-// Measured on a B200 (6.56 TB/s copy), 8 KV heads of dim 64 with 8 query heads each: 32 sequences of
+// Measured on a B200 (6.56 TB/s copy), from a CUDA graph, 8 KV heads of dim 64 with 8 query heads each: 32 sequences of
 // 129 to 16384 slots (542 MB) 96 us, 5.7 TB/s; 256 windows of 128 (72 MB) 16 us, 4.5 TB/s, bound by the
 // dependent steps of one short walk a warp; one window 4.5 us, all of it latency; one sequence of
 // 131072 slots with its weights (277 MB) 69 us, of which 54 the attention (268 MB, and 34 MB of scores
@@ -124,7 +124,8 @@ __device__ __forceinline__ int64_t warp_prefix(int64_t x, int lane) {  // exclus
   return y - x;
 }
 
-// Blocks that share `total` units: two units a warp at least, so that none of them is without any.
+// Blocks that share `total` units, two for each warp: a warp is without any only where there are fewer
+// than kWarps of them in all.
 __device__ __forceinline__ int active_blocks(int64_t total, int blocks) {
   const int64_t n = (total + 2 * kWarps - 1) / (2 * kWarps);
   return n < blocks ? (int)n : blocks;

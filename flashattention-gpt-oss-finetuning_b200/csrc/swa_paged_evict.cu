@@ -18,8 +18,9 @@
 // moves and its length stays, like one whose length is out of range.  Every block looks through the
 // sequence's whole table, so that all its heads decide alike without a word between them.
 //
-// Measured on a B200: 4 x 8 heads of 16384 to 32768 slots cut to 4096 (57 MB of rows move): select 20 us,
-// move 16; 64 x 4 heads of some 1080 slots cut to 1024, in one kernel, 12 us.
+// Measured on a B200, from a CUDA graph: 4 x 8 heads of 16384 to 32768 slots cut to 4096 (57 MB of rows
+// move) 34 us (with cold caches select 20, move 17); 64 x 4 heads of dim 128 with some 1080 slots cut to
+// 1024, in one kernel, 13 us (cold 17).
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -38,7 +39,8 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 256;
 constexpr int kDigits = 4;
 constexpr int kMaxCluster = 8;
-constexpr int kMaxKeys = 24576;  // keys a block keeps (96 KB, two blocks an SM); more are read again from memory
+// keys a block keeps, 96 KB (two blocks an SM up to 23552 keys, one beyond); more are read again from memory
+constexpr int kMaxKeys = 24576;
 constexpr int kAhead = 8;        // slots whose loads a thread has under way
 constexpr int kMoveThreads = 256;
 
@@ -320,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 2) select_kernel(const __grid_consta
 
 // blockIdx.y strides over (sequence, KV head), blockIdx.x over the pieces of its moves; then the
 // lengths.  One piece a thread and full occupancy: two a thread at half of it are 3 us slower where
-// 57 MB move (18 us, 3.2 TB/s in scattered rows of 128 bytes).
+// 57 MB move (17 us with cold caches, 3.4 TB/s in scattered rows of 128 bytes).
 __global__ void __launch_bounds__(kMoveThreads, 8) move_kernel(const __grid_constant__ EvictParams p) {
   sm100::pdl_wait();
   const int heads = p.c.batch * p.c.n_kv_heads;
@@ -336,8 +338,8 @@ __global__ void __launch_bounds__(kMoveThreads, 8) move_kernel(const __grid_cons
 }
 
 // Blocks per (sequence, KV head): as many as fit beside one another (two an SM), of no less than
-// 2048 slots each; more where a block could not keep its keys.  (4 x 8 heads of 32768 slots, eviction
-// in all: 8 blocks a head 43 us, 4 46.)
+// 2048 slots each; more where a block could not keep its keys.  (4 x 8 heads of 32768 slots, calls with
+// the copy that restores the weights, when this was chosen: 8 blocks a head 43 us, 4 46.)
 int cluster_size(const PagedParams& c) {
   const int64_t heads = (int64_t)c.batch * c.n_kv_heads, slots = (int64_t)c.max_pages * c.page_size;
   int size = 1;
@@ -394,7 +396,8 @@ cudaError_t launch_paged_evict(const PagedParams& c, const SwaPagedEvictArgs& a,
   const int cluster = cluster_size(c);
   const int64_t slots = (int64_t)c.max_pages * c.page_size;
   // Few moves, at most four pieces a thread, of heads that fit in a cluster: one kernel does it all
-  // (calls one after the other: 8 heads of one sequence 12.8 us, 14.0 with two kernels; 64 x 4 heads of dim 128
+  // (calls one after the other, when this was chosen: 8 heads of one sequence 12.8 us, 14.0 with two kernels;
+  // with the copy that restores the weights, 2 us on the GPU and a launch, 64 x 4 heads of dim 128
   // 22.1 and 22.6).
   p.all_here = cluster == 1 && c.n_kv_heads <= kMaxCluster && (int64_t)p.most * p.pieces <= 4 * kThreads;
   const int64_t per = (slots + cluster * kThreads - 1) / (cluster * kThreads) * kThreads;
