@@ -63,8 +63,9 @@ class PagedKVCache:
 
     The tensors are the caller's: their values may change between calls (also under a captured
     graph), the cache itself holds only their addresses.  A page number outside the pool or a
-    length beyond the table is not followed: that sequence's output is NaN, its rows
-    of ``weights_out`` stay, an eviction leaves it as it is, an append writes only tokens whose own page is in range, and :meth:`check` raises."""
+    length beyond the table is not followed: that sequence's output is NaN, its rows of
+    ``weights_out`` stay, an eviction leaves it as it is, an append writes only tokens whose own
+    page is in range, and :meth:`check` raises."""
 
     def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                  seq_lens: torch.Tensor, weights: Optional[torch.Tensor] = None,
